@@ -4,7 +4,8 @@ The decode hot path of fastserve (kernels/kv_attention.py, engine/kv_cache.py, i
 re-implemented as hand-written HIP kernels behind a C ABI (include/bpt_amd.h, built into libbpt_amd.so)
 with a thin PyTorch-ROCm host layer: paged FP8 / INT8 / BF16 pools (paged_attention, kv_cache) and
 contiguous KIVI caches (kivi: fastserve's kernels/kv_attention.py call surface), and the fused RMSNorm +
-per-token INT8 quantizer (norm_quant: kernels/norm_quant.py). Importing needs no GPU; the library loads on first use and raises if
+per-token INT8 quantizer (norm_quant: kernels/norm_quant.py), and rotary positions on the way into the paged cache
+(rotary). Importing needs no GPU; the library loads on first use and raises if
 it has not been built.
 """
 
@@ -21,6 +22,7 @@ from .paged_attention import (
     paged_prepare,
     quantize_append,
 )
+from .rotary import rotary_append, rotary_embed
 
 __all__ = [
     "cascade_decode_attention",
@@ -36,4 +38,6 @@ __all__ = [
     "paged_prepare",
     "quantize_append",
     "rms_norm_int8",
+    "rotary_append",
+    "rotary_embed",
 ]

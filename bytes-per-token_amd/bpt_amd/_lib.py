@@ -281,6 +281,52 @@ class NormQuantArgs(ctypes.Structure):
     ]
 
 
+class RotaryArgs(ctypes.Structure):
+    _fields_ = [
+        ("struct_size", ctypes.c_uint32),
+        ("x_dtype", _i32),
+        ("norm_dtype", _i32),
+        ("positions_dtype", _i32),
+        ("batch", _i32),
+        ("num_queries", _i32),
+        ("num_q_heads", _i32),
+        ("num_k_heads", _i32),
+        ("head_dim", _i32),
+        ("rotary_dim", _i32),
+        ("num_axes", _i32),
+        ("interleaved", _i32),
+        ("scaling", ctypes.c_float),
+        ("eps", ctypes.c_float),
+        ("q", _vp),
+        ("q_stride_b", _i64),
+        ("q_stride_q", _i64),
+        ("q_stride_h", _i64),
+        ("k", _vp),
+        ("k_stride_b", _i64),
+        ("k_stride_q", _i64),
+        ("k_stride_h", _i64),
+        ("q_out", _vp),
+        ("q_out_stride_b", _i64),
+        ("q_out_stride_q", _i64),
+        ("q_out_stride_h", _i64),
+        ("k_out", _vp),
+        ("k_out_stride_b", _i64),
+        ("k_out_stride_q", _i64),
+        ("k_out_stride_h", _i64),
+        ("q_norm", _vp),
+        ("k_norm", _vp),
+        ("inv_freq", _vp),
+        ("positions", _vp),
+        ("pos_stride_a", _i64),
+        ("pos_stride_b", _i64),
+        ("pos_stride_q", _i64),
+        ("pair_axis", ctypes.c_uint8 * 128),
+    ]
+
+
+ROTARY_ARGS_SIZE = ctypes.sizeof(RotaryArgs)
+
+
 # Every symbol include/bpt_amd.h declares, with its ctypes signature.
 SIGNATURES = {
     "bpt_decode_plan": (
@@ -301,6 +347,8 @@ SIGNATURES = {
     "bpt_rms_norm_int8": (_i32, [ctypes.POINTER(NormQuantArgs), _vp]),
     "bpt_kivi_quantize": (_i32, [ctypes.POINTER(KiviQuantArgs), _vp]),
     "bpt_paged_prepare": (_i32, [ctypes.POINTER(PrepareArgs), _vp]),
+    "bpt_rotary_embed": (_i32, [ctypes.POINTER(RotaryArgs), _vp]),
+    "bpt_rotary_append": (_i32, [ctypes.POINTER(RotaryArgs), ctypes.POINTER(AppendArgs), _vp]),
     "bpt_last_error": (ctypes.c_char_p, []),
     "bpt_abi_version": (_i32, []),
     "bpt_source_hash": (ctypes.c_char_p, []),
@@ -312,7 +360,7 @@ SIGNATURES = {
     "bpt_copy_probe": (_i32, [_vp, _vp, ctypes.c_uint64, _vp]),
 }
 
-ABI_VERSION = 13
+ABI_VERSION = 14
 
 
 class BptError(RuntimeError):

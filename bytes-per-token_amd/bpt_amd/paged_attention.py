@@ -19,6 +19,7 @@ Conventions, as in fastserve (paths relative to its src/fastserve/):
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 
 import torch
@@ -55,6 +56,14 @@ def kv_dtype_code(dtype: torch.dtype) -> int:
 def _stream(device: torch.device) -> int:
     """The device's current HIP stream as an integer handle (without the object that torch.cuda.current_stream makes)."""
     return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if device.index is None else device.index)
+
+
+_HERE = contextlib.nullcontext()
+
+
+def _on_device(device: torch.device):
+    """Makes `device` the current one where it is not: kernels are launched on the current device."""
+    return _HERE if device.index is None or device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 def _scale_layout(k_scale, v_scale, kv_code: int, pool_shape) -> tuple[int, tuple[int, int, int]]:

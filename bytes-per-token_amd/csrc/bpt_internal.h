@@ -350,6 +350,42 @@ struct NormQuantParams {
   int x_dtype, w_dtype;
 };
 
+// Launch-ready form of bpt_rotary_args, with the pool's fields of bpt_append_args when the keys go into one.
+constexpr int kRotaryMaxDim = 256;
+constexpr int kRotaryMaxAxes = 8;
+constexpr int kRotaryMaxAngles = 1024;  // pairs whose angles a workgroup holds in LDS
+struct RotaryParams {
+  const void* q;
+  const void* k;
+  const void* v;
+  void* q_out;
+  void* k_out;
+  int64_t q_sb, q_sq, q_sh, k_sb, k_sq, k_sh;  // elements; v shares k's
+  int64_t qo_sb, qo_sq, qo_sh, ko_sb, ko_sq, ko_sh;
+  const void* q_norm;
+  const void* k_norm;
+  const float* inv_freq;
+  const void* positions;
+  int64_t pos_sa, pos_sb, pos_sq;
+  int64_t tokens;  // B * Q
+  int Q, Hq, Hk, D, rot, interleaved, pos_i64, norm_dtype;
+  int tokens_per_group;  // tokens of one workgroup
+  int log_lanes;         // log2 of the lanes that hold a row
+  int vec;               // rows can be loaded and stored 8 channels at a time
+  float scaling, eps;
+  const void* blocks;
+  const void* offsets;
+  int64_t s_sb, s_sq;
+  uint8_t* kc;
+  uint8_t* vc;
+  int64_t kv_sblk, kv_stok, kv_shead;  // bytes
+  float* ks;
+  float* vs;
+  int64_t sc_sblk, sc_stok, sc_shead;  // elements
+  int P, num_blocks, slot_i64;
+  uint8_t axis[kRotaryMaxDim / 2];  // the axis of positions that turns each pair
+};
+
 // KIVI storage formats of bpt_kivi_args.bits / kv_dtype.
 constexpr int kKivi4 = 0;
 constexpr int kKivi8 = 1;
@@ -383,6 +419,7 @@ hipError_t launch_kivi(const KiviParams& p, int fmt, hipStream_t stream);
 // Any even head dim up to 256 and float32 bits-16 caches: one workgroup per (sequence, KV head, split).
 hipError_t launch_kivi_any(const KiviParams& p, int fmt, hipStream_t stream);
 hipError_t launch_norm_quant(const NormQuantParams& p, bool vec8, hipStream_t stream);
+hipError_t launch_rotary(const RotaryParams& p, int x_dtype, bool pool, int kv_dtype, int scale_kind, hipStream_t stream);
 hipError_t launch_kivi_quantize(const KiviQuantParams& p, hipStream_t stream);
 hipError_t launch_paged_prepare(const PrepareParams& p, hipStream_t stream);
 hipError_t launch_append(const AppendParams& p, int kv_dtype, int scale_kind, int head_dim, hipStream_t stream);

@@ -2,6 +2,7 @@
 //
 // Argument checks run on the host before anything is launched and report BPT_ERR_INVALID_ARGUMENT with a
 // message; nothing here reads device memory, so every call stays asynchronous and graph-capturable.
+#include <algorithm>
 #include <cmath>
 #include <cstdarg>
 #include <cstdio>
@@ -983,6 +984,157 @@ int bpt_paged_append_decode(const bpt_append_args* append, const bpt_decode_args
     if (e != hipSuccess) return hip_fail(fn, e);
   }
   return paged_decode(decode, stream, {}, fn);
+}
+
+namespace {
+
+// Whether rows of `elem`-byte channels can be loaded 8 at a time.
+bool rows_aligned(const void* p, int64_t sb, int64_t sq, int64_t sh, int elem) {
+  return !p || aligned_to(p, sb, sq, sh, elem);
+}
+
+// Checks a rotary call's arguments on the host and fills its launch parameters, the pool's fields aside. *empty: no token.
+int rotary_params(const bpt_rotary_args* a, bool pool, bpt::RotaryParams* out, bool* empty, const char* fn) {
+  if (!a) return fail(BPT_ERR_INVALID_ARGUMENT, "%s: args is NULL", fn);
+  if (a->struct_size != sizeof(bpt_rotary_args))
+    return fail(BPT_ERR_INVALID_ARGUMENT, "%s: struct_size %u != %zu (stale binding)", fn, a->struct_size,
+                sizeof(bpt_rotary_args));
+  if (a->x_dtype < BPT_F_BF16 || a->x_dtype > BPT_F_F32)
+    return fail(BPT_ERR_INVALID_ARGUMENT, "%s: q and k must be bf16, f16 or f32", fn);
+  if ((a->q_norm || a->k_norm) && (a->norm_dtype < BPT_F_BF16 || a->norm_dtype > BPT_F_F32))
+    return fail(BPT_ERR_INVALID_ARGUMENT, "%s: norm weights must be bf16, f16 or f32", fn);
+  if (a->positions_dtype != BPT_IDX_I32 && a->positions_dtype != BPT_IDX_I64)
+    return fail(BPT_ERR_INVALID_ARGUMENT, "%s: positions must be int32 or int64", fn);
+  if (a->batch < 0 || a->num_queries < 0 || a->num_q_heads < 0 || a->num_k_heads < 0)
+    return fail(BPT_ERR_INVALID_ARGUMENT, "%s: batch, num_queries and heads must be >= 0", fn);
+  if (a->num_q_heads > (1 << 16) || a->num_k_heads > (1 << 16))
+    return fail(BPT_ERR_INVALID_ARGUMENT, "%s: too many heads", fn);
+  if (a->head_dim < 2 || a->head_dim > bpt::kRotaryMaxDim || a->head_dim % 2)
+    return fail(BPT_ERR_INVALID_ARGUMENT, "%s: head_dim %d not supported (an even number up to %d)", fn, a->head_dim,
+                bpt::kRotaryMaxDim);
+  if (a->rotary_dim < 2 || a->rotary_dim > a->head_dim || a->rotary_dim % 2)
+    return fail(BPT_ERR_INVALID_ARGUMENT, "%s: rotary_dim %d must be even, from 2 to head_dim %d", fn, a->rotary_dim,
+                a->head_dim);
+  if (a->num_axes < 1 || a->num_axes > bpt::kRotaryMaxAxes)
+    return fail(BPT_ERR_INVALID_ARGUMENT, "%s: num_axes must be 1 to %d", fn, bpt::kRotaryMaxAxes);
+  for (int i = 0; i < a->rotary_dim / 2; ++i)
+    if (a->pair_axis[i] >= a->num_axes)
+      return fail(BPT_ERR_INVALID_ARGUMENT, "%s: pair %d follows axis %d of %d", fn, i, a->pair_axis[i], a->num_axes);
+  if (!std::isfinite(a->scaling)) return fail(BPT_ERR_INVALID_ARGUMENT, "%s: scaling must be finite", fn);
+  if (!(a->eps >= 0.0f) || !std::isfinite(a->eps))
+    return fail(BPT_ERR_INVALID_ARGUMENT, "%s: eps must be finite and not negative", fn);
+  const int64_t tokens = (int64_t)a->batch * a->num_queries;
+  *empty = tokens == 0 || a->num_q_heads + a->num_k_heads == 0;
+  if (*empty) return BPT_OK;
+  if (tokens > 0x7fffffffLL) return fail(BPT_ERR_INVALID_ARGUMENT, "%s: too many tokens", fn);
+  if ((a->num_q_heads && (!a->q || !a->q_out)) || (a->num_k_heads && (!a->k || (!pool && !a->k_out))) || !a->inv_freq ||
+      !a->positions)
+    return fail(BPT_ERR_INVALID_ARGUMENT, "%s: rows, outputs, inv_freq and positions must be non-NULL", fn);
+
+  bpt::RotaryParams p{};
+  p.q = a->q;
+  p.q_sb = a->q_stride_b;
+  p.q_sq = a->q_stride_q;
+  p.q_sh = a->q_stride_h;
+  p.k = a->k;
+  p.k_sb = a->k_stride_b;
+  p.k_sq = a->k_stride_q;
+  p.k_sh = a->k_stride_h;
+  p.q_out = a->q_out;
+  p.qo_sb = a->q_out_stride_b;
+  p.qo_sq = a->q_out_stride_q;
+  p.qo_sh = a->q_out_stride_h;
+  p.k_out = a->k_out;
+  p.ko_sb = a->k_out_stride_b;
+  p.ko_sq = a->k_out_stride_q;
+  p.ko_sh = a->k_out_stride_h;
+  p.q_norm = a->q_norm;
+  p.k_norm = a->k_norm;
+  p.norm_dtype = a->norm_dtype;
+  p.inv_freq = a->inv_freq;
+  p.positions = a->positions;
+  p.pos_sa = a->pos_stride_a;
+  p.pos_sb = a->pos_stride_b;
+  p.pos_sq = a->pos_stride_q;
+  p.pos_i64 = a->positions_dtype == BPT_IDX_I64;
+  p.tokens = tokens;
+  p.Q = a->num_queries;
+  p.Hq = a->num_q_heads;
+  p.Hk = a->num_k_heads;
+  p.D = a->head_dim;
+  p.rot = a->rotary_dim;
+  p.interleaved = a->interleaved != 0;
+  p.scaling = a->scaling;
+  p.eps = a->eps;
+  const int half = a->rotary_dim / 2, elem = float_bytes(a->x_dtype);
+  for (int i = 0; i < half; ++i) p.axis[i] = a->pair_axis[i];
+  // A lane holds 8 pairs, or 16 of the channels behind them.
+  const int units = std::max((half + 7) / 8 + (a->head_dim - a->rotary_dim + 15) / 16, (a->head_dim + 15) / 16);
+  p.log_lanes = log2i(units);
+  p.vec = half % 8 == 0 && a->head_dim % 16 == 0 &&
+          (!a->num_q_heads || (rows_aligned(a->q, a->q_stride_b, a->q_stride_q, a->q_stride_h, elem) &&
+                               rows_aligned(a->q_out, a->q_out_stride_b, a->q_out_stride_q, a->q_out_stride_h, elem))) &&
+          (!a->num_k_heads || (rows_aligned(a->k, a->k_stride_b, a->k_stride_q, a->k_stride_h, elem) &&
+                               (pool || rows_aligned(a->k_out, a->k_out_stride_b, a->k_out_stride_q, a->k_out_stride_h, elem))));
+  const int rows = a->num_q_heads + (pool ? 2 : 1) * a->num_k_heads, at_once = 256 >> p.log_lanes;
+  const int64_t fill = (at_once + rows - 1) / rows;  // tokens that give every thread a row
+  const int64_t most = bpt::kRotaryMaxAngles / half;
+  p.tokens_per_group = (int)std::max<int64_t>(1, std::min(fill, most));
+  *out = p;
+  return BPT_OK;
+}
+
+}  // namespace
+
+int bpt_rotary_embed(const bpt_rotary_args* a, void* stream) {
+  const char* fn = "bpt_rotary_embed";
+  bpt::RotaryParams p;
+  bool empty;
+  int rc = rotary_params(a, false, &p, &empty, fn);
+  if (rc || empty) return rc;
+  hipError_t e = bpt::launch_rotary(p, a->x_dtype, false, 0, 0, (hipStream_t)stream);
+  if (e != hipSuccess) return hip_fail(fn, e);
+  return BPT_OK;
+}
+
+int bpt_rotary_append(const bpt_rotary_args* a, const bpt_append_args* append, void* stream) {
+  const char* fn = "bpt_rotary_append";
+  bpt::RotaryParams p;
+  bpt::AppendParams w;
+  bool empty, no_rows;
+  int rc = rotary_params(a, true, &p, &empty, fn);
+  if (rc) return rc;
+  rc = append_params(append, &w, &no_rows, fn);
+  if (rc) return rc;
+  if (append->batch != a->batch || append->num_queries != a->num_queries || append->num_kv_heads != a->num_k_heads ||
+      append->head_dim != a->head_dim || append->src_dtype != a->x_dtype)
+    return fail(BPT_ERR_INVALID_ARGUMENT, "%s: both halves must describe the same keys", fn);
+  if (empty || no_rows) return BPT_OK;
+  if (append->k != a->k || append->new_stride_b != a->k_stride_b || append->new_stride_q != a->k_stride_q ||
+      append->new_stride_h != a->k_stride_h)
+    return fail(BPT_ERR_INVALID_ARGUMENT, "%s: both halves must describe the same keys", fn);
+  p.v = append->v;
+  p.vec = p.vec && rows_aligned(append->v, p.k_sb, p.k_sq, p.k_sh, float_bytes(a->x_dtype));
+  p.blocks = w.blocks;
+  p.offsets = w.offsets;
+  p.s_sb = w.s_sb;
+  p.s_sq = w.s_sq;
+  p.slot_i64 = w.slot_i64;
+  p.kc = w.kc;
+  p.vc = w.vc;
+  p.kv_sblk = w.kv_sblk;
+  p.kv_stok = w.kv_stok;
+  p.kv_shead = w.kv_shead;
+  p.ks = w.ks;
+  p.vs = w.vs;
+  p.sc_sblk = w.sc_sblk;
+  p.sc_stok = w.sc_stok;
+  p.sc_shead = w.sc_shead;
+  p.P = w.P;
+  p.num_blocks = w.num_blocks;
+  hipError_t e = bpt::launch_rotary(p, a->x_dtype, true, append->kv_dtype, append->scale_kind, (hipStream_t)stream);
+  if (e != hipSuccess) return hip_fail(fn, e);
+  return BPT_OK;
 }
 
 int bpt_fp8_decode_table(float* out256, void* stream) {

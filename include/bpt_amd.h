@@ -29,6 +29,8 @@
  *                        integration/kv_cache.py:139-158 QuantizedKVCache._append quantizes completed groups.
  *   bpt_rms_norm_int8    kernels/norm_quant.py:43-109 rms_norm_int8 (kernel 1), defined by
  *                        kernels/reference.py:44-55: RMSNorm fused with per-token INT8 quantization.
+ *   bpt_rotary_embed     engine/rope.py and the per-head norms ahead of engine/model.py:52-74's attend, one launch.
+ *   bpt_rotary_append    the same, with the write half of the cache's attend (bpt_quant_append).
  */
 #ifndef BPT_AMD_H
 #define BPT_AMD_H
@@ -40,7 +42,7 @@
 extern "C" {
 #endif
 
-#define BPT_ABI_VERSION 13
+#define BPT_ABI_VERSION 14
 
 /* return codes */
 #define BPT_OK 0
@@ -359,6 +361,45 @@ typedef struct {
   float* scale;
 } bpt_norm_quant_args;
 
+/*
+ * Rotary positions: queries and keys normalised per head (optional) and rotated, float32 arithmetic, rounded once.
+ * For the rotary_dim / 2 pairs i of a row's leading channels, with t = positions[pair_axis[i], b, q] * inv_freq[i] (the
+ * angle in float64):  (a, b) -> scaling * (a cos t - b sin t, a sin t + b cos t).  The pairs are channels (i, i +
+ * rotary_dim / 2), or (2 i, 2 i + 1) with `interleaved`; channels past rotary_dim are not rotated. With norm weights,
+ * x -> x * rsqrt(mean(x^2) + eps) * weight over the head's channels comes first.
+ *   q, k        [B, Q, Hq, D], [B, Q, Hk, D] (strides {q,k}_stride_{b,q,h}; channel stride 1), x_dtype BF16 / F16 / F32;
+ *               num_k_heads 0: no keys
+ *   q/k_out     the same shapes and type, strides {q,k}_out_stride_{b,q,h}; may be the inputs themselves (in place),
+ *               but may not overlap them in part
+ *   q/k_norm    [D] norm_dtype, or NULL: not normalised
+ *   inv_freq    float32 [rotary_dim / 2]
+ *   positions   [num_axes, B, Q] int32 / int64 (strides pos_stride_{a,b,q}), any integers
+ *   pair_axis   the axis of each pair, below num_axes (at most 8)
+ * D and rotary_dim even, rotary_dim <= D <= 256. Rows whose strides are not multiples of 16 bytes, and sizes that are not
+ * multiples of 16 channels, take element-wise loads.
+ */
+typedef struct {
+  uint32_t struct_size; /* sizeof(bpt_rotary_args) */
+  int32_t x_dtype, norm_dtype;  /* bpt_float_dtype */
+  int32_t positions_dtype;      /* bpt_index_dtype */
+  int32_t batch, num_queries, num_q_heads, num_k_heads, head_dim, rotary_dim, num_axes, interleaved;
+  float scaling, eps;
+  const void* q;
+  int64_t q_stride_b, q_stride_q, q_stride_h;
+  const void* k;
+  int64_t k_stride_b, k_stride_q, k_stride_h;
+  void* q_out;
+  int64_t q_out_stride_b, q_out_stride_q, q_out_stride_h;
+  void* k_out;
+  int64_t k_out_stride_b, k_out_stride_q, k_out_stride_h;
+  const void* q_norm;
+  const void* k_norm;
+  const float* inv_freq;
+  const void* positions;
+  int64_t pos_stride_a, pos_stride_b, pos_stride_q;
+  uint8_t pair_axis[128];
+} bpt_rotary_args;
+
 /* ---- entry points ------------------------------------------------------------------------------- */
 
 /* Host-only: validate args, fill chunk_tokens / grid_groups, report the workspace and counter sizes in
@@ -410,6 +451,17 @@ int bpt_kivi_quantize(const bpt_kivi_quant_args* args, void* stream);
 
 /* RMSNorm fused with per-token INT8 quantization (one launch). */
 int bpt_rms_norm_int8(const bpt_norm_quant_args* args, void* stream);
+
+/* Queries and keys normalised and rotated by their positions: one launch. No counterpart among the reference's kernels; its
+ * model does this in torch ahead of the cache's attend (engine/model.py:52-74, engine/rope.py). */
+int bpt_rotary_embed(const bpt_rotary_args* args, void* stream);
+
+/* bpt_rotary_embed whose keys go into the paged pools, with the values, as bpt_quant_append stores them (from the rotated
+ * keys in float32, not rounded to x_dtype first): one launch. `append` gives the keys' and values' rows, slots and pools;
+ * its batch, num_queries, num_kv_heads, head_dim, src_dtype and k have to be those of `args`, whose k_out is not used. The
+ * write slots of a call have to be distinct: of two rows with one slot, either may be left there, in parts. Every argument
+ * is checked before anything is launched. */
+int bpt_rotary_append(const bpt_rotary_args* args, const bpt_append_args* append, void* stream);
 
 /* Thread-local message of the last failing call ("" when none). */
 const char* bpt_last_error(void);

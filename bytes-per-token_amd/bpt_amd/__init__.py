@@ -5,13 +5,14 @@ re-implemented as hand-written HIP kernels behind a C ABI (include/bpt_amd.h, bu
 with a thin PyTorch-ROCm host layer: paged FP8 / INT8 / BF16 pools (paged_attention, kv_cache) and
 contiguous KIVI caches (kivi: fastserve's kernels/kv_attention.py call surface), and the fused RMSNorm +
 per-token INT8 quantizer (norm_quant: kernels/norm_quant.py), and rotary positions on the way into the paged cache
-(rotary). Importing needs no GPU; the library loads on first use and raises if
+(rotary) and attention with masked and shaped scores over it (masked_attention). Importing needs no GPU; the library loads on first use and raises if
 it has not been built.
 """
 
 from . import kivi
 from .cascade import cascade_decode_attention
 from .kv_cache import OutOfBlocksError, PagedMeta, PagedQuantKVCache
+from .masked_attention import masked_plan, paged_masked_attention
 from .norm_quant import rms_norm_int8
 from .paged_attention import (
     decode_kernel_name,
@@ -33,8 +34,10 @@ __all__ = [
     "decode_plan",
     "kivi",
     "kv_read_bytes",
+    "masked_plan",
     "paged_append_decode",
     "paged_decode_attention",
+    "paged_masked_attention",
     "paged_prepare",
     "quantize_append",
     "rms_norm_int8",

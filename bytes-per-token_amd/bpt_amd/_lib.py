@@ -281,6 +281,23 @@ class NormQuantArgs(ctypes.Structure):
     ]
 
 
+class MaskArgs(ctypes.Structure):
+    _fields_ = [
+        ("struct_size", ctypes.c_uint32),
+        ("softcap", ctypes.c_float),
+        ("window", _i32),
+        ("max_prefix", _i32),
+        ("slopes", _vp),
+        ("prefix_lens", _vp),
+        ("starts", _vp),
+        ("start_stride_b", _i64),
+        ("start_stride_q", _i64),
+    ]
+
+
+MASK_ARGS_SIZE = ctypes.sizeof(MaskArgs)
+
+
 class RotaryArgs(ctypes.Structure):
     _fields_ = [
         ("struct_size", ctypes.c_uint32),
@@ -347,6 +364,11 @@ SIGNATURES = {
     "bpt_rms_norm_int8": (_i32, [ctypes.POINTER(NormQuantArgs), _vp]),
     "bpt_kivi_quantize": (_i32, [ctypes.POINTER(KiviQuantArgs), _vp]),
     "bpt_paged_prepare": (_i32, [ctypes.POINTER(PrepareArgs), _vp]),
+    "bpt_masked_plan": (
+        _i32,
+        [ctypes.POINTER(DecodeArgs), ctypes.POINTER(MaskArgs), ctypes.POINTER(ctypes.c_size_t), ctypes.POINTER(ctypes.c_size_t)],
+    ),
+    "bpt_paged_masked": (_i32, [ctypes.POINTER(DecodeArgs), ctypes.POINTER(MaskArgs), _vp]),
     "bpt_rotary_embed": (_i32, [ctypes.POINTER(RotaryArgs), _vp]),
     "bpt_rotary_append": (_i32, [ctypes.POINTER(RotaryArgs), ctypes.POINTER(AppendArgs), _vp]),
     "bpt_last_error": (ctypes.c_char_p, []),

@@ -350,6 +350,41 @@ struct NormQuantParams {
   int x_dtype, w_dtype;
 };
 
+// Launch-ready form of a bpt_paged_masked call (cache strides in bytes, others in elements).
+constexpr float kMaskedPlainCap = 369.0f;  // largest cap (log2 units) that takes the plain form of tanh: 256 in natural ones
+struct MaskedParams {
+  const void* q;
+  int64_t q_sb, q_sq, q_sh;
+  const uint8_t* k;
+  const uint8_t* v;
+  int64_t kv_sblk, kv_stok, kv_shead;
+  const float* ks;
+  const float* vs;
+  int64_t sc_sblk, sc_stok, sc_shead;
+  const void* table;
+  int64_t table_sb;
+  const int32_t* lens;
+  void* out;
+  int64_t o_sb, o_sq, o_sh;
+  float* lse_out;
+  const float* slopes;         // [Hq] or NULL
+  const int32_t* prefix_lens;  // [B] or NULL
+  const int32_t* starts;       // [B, Q] or NULL
+  int64_t st_sb, st_sq;
+  float* ws_out;       // [segments, max_pieces, live_rows, D] normalized partials
+  float* ws_lse;       // [segments, max_pieces, live_rows] their log2-sum-exp
+  unsigned* counters;  // [segments] arrivals; zero between calls
+  int Q, Hq, Hkv, G, P, logP, num_blocks, len_cap, table_i64, out_dtype;
+  int window;      // 0: none
+  int max_prefix;  // prefix lengths above it are cut to it
+  int tiles;       // row tiles of a KV head
+  int live_rows;   // rows of the largest tile
+  int piece;       // steps of a piece
+  int max_pieces;  // pieces of the longest tile
+  float qscale;    // of raw products: log2 units, or with a cap the argument of its exponential
+  float cap;       // log2 units; 0: none
+};
+
 // Launch-ready form of bpt_rotary_args, with the pool's fields of bpt_append_args when the keys go into one.
 constexpr int kRotaryMaxDim = 256;
 constexpr int kRotaryMaxAxes = 8;
@@ -419,6 +454,11 @@ hipError_t launch_kivi(const KiviParams& p, int fmt, hipStream_t stream);
 // Any even head dim up to 256 and float32 bits-16 caches: one workgroup per (sequence, KV head, split).
 hipError_t launch_kivi_any(const KiviParams& p, int fmt, hipStream_t stream);
 hipError_t launch_norm_quant(const NormQuantParams& p, bool vec8, hipStream_t stream);
+hipError_t launch_masked_bf16(const MaskedParams& p, bool q_split, int rt, bool many, int grid, hipStream_t stream);
+hipError_t launch_masked_fp8_head(const MaskedParams& p, bool q_split, int rt, bool many, int grid, hipStream_t stream);
+hipError_t launch_masked_fp8_token(const MaskedParams& p, bool q_split, int rt, bool many, int grid, hipStream_t stream);
+hipError_t launch_masked_int8_head(const MaskedParams& p, bool q_split, int rt, bool many, int grid, hipStream_t stream);
+hipError_t launch_masked_int8_token(const MaskedParams& p, bool q_split, int rt, bool many, int grid, hipStream_t stream);
 hipError_t launch_rotary(const RotaryParams& p, int x_dtype, bool pool, int kv_dtype, int scale_kind, hipStream_t stream);
 hipError_t launch_kivi_quantize(const KiviQuantParams& p, hipStream_t stream);
 hipError_t launch_paged_prepare(const PrepareParams& p, hipStream_t stream);

@@ -988,6 +988,161 @@ int bpt_paged_append_decode(const bpt_append_args* append, const bpt_decode_args
 
 namespace {
 
+struct MaskedPlan {
+  int rt;     // 16-row tiles of a wave
+  bool many;  // the kernel that shares tiles of 64 rt rows among four waves, else one wave holds all rows
+  int grid;
+  size_t workspace, counters, ws_out_floats;
+};
+
+// Checks a masked call on the host and fills its launch parameters, the buffers aside.
+int masked_setup(const bpt_decode_args* a, const bpt_mask_args* m, const char* fn, bpt::MaskedParams* out, MaskedPlan* plan) {
+  Plan pl;
+  int rc = make_plan(a, &pl, false);  // the checks of the shapes that both calls share
+  if (rc) return rc;
+  if (!m) return fail(BPT_ERR_INVALID_ARGUMENT, "%s: mask is NULL", fn);
+  if (m->struct_size != sizeof(bpt_mask_args))
+    return fail(BPT_ERR_INVALID_ARGUMENT, "%s: struct_size %u != %zu (stale binding)", fn, m->struct_size,
+                sizeof(bpt_mask_args));
+  if (a->q_dtype == BPT_F_F32) return fail(BPT_ERR_INVALID_ARGUMENT, "%s: q must be bf16 or f16", fn);
+  if (a->num_splits || a->flags || a->len_offset || a->merge_out || a->merge_lse)
+    return fail(BPT_ERR_INVALID_ARGUMENT, "%s: takes no num_splits, flags, len_offset or partial to merge", fn);
+  if (!(m->softcap >= 0.0f) || !std::isfinite(m->softcap))
+    return fail(BPT_ERR_INVALID_ARGUMENT, "%s: softcap must be positive and finite (0: none)", fn);
+  if (m->window < 0) return fail(BPT_ERR_INVALID_ARGUMENT, "%s: window must be at least 1 (0: none)", fn);
+  if (m->max_prefix < 0) return fail(BPT_ERR_INVALID_ARGUMENT, "%s: max_prefix must be >= 0", fn);
+  const int eb = a->kv_dtype == BPT_KV_BF16 ? 2 : 1;
+  if (a->kv_stride_token < 0 || a->kv_stride_token * eb >= (int64_t(1) << 27))
+    return fail(BPT_ERR_INVALID_ARGUMENT, "%s: 16 tokens of a page must lie within 2 GiB", fn);
+
+  bpt::MaskedParams p{};
+  p.Q = a->num_queries;
+  p.Hq = a->num_q_heads;
+  p.Hkv = a->num_kv_heads;
+  p.G = a->num_q_heads / a->num_kv_heads;
+  p.P = a->page_size;
+  p.logP = log2i(a->page_size);
+  p.num_blocks = a->num_blocks;
+  const int64_t reach = (int64_t)a->max_blocks_per_seq * a->page_size;
+  p.len_cap = (int)std::min<int64_t>(a->max_context, reach);
+  p.window = m->window >= p.len_cap ? 0 : m->window;  // a window of all tokens hides none
+  p.max_prefix = m->prefix_lens ? std::min(m->max_prefix, p.len_cap) : 0;
+  const double log2e = 1.4426950408889634, scale = (double)a->sm_scale * log2e;
+  p.cap = (float)(m->softcap * log2e);
+  p.qscale = (float)(m->softcap > 0.0f ? 2.0 * scale / m->softcap : scale);
+  if (!std::isfinite(p.qscale) || !std::isfinite(2.0f * p.cap))
+    return fail(BPT_ERR_INVALID_ARGUMENT, "%s: sm_scale %g and softcap %g are out of range", fn, a->sm_scale, m->softcap);
+
+  // Rows: one wave holds up to 32 (it reads its tokens' keys and values straight into registers), else four waves share
+  // tiles of 64 or 128 whose operands they convert once between them.
+  const int rows = pl.rows;
+  plan->many = rows > 32;
+  plan->rt = plan->many ? (rows > 64 ? 2 : 1) : (rows > 16 ? 2 : 1);
+  const int tile = plan->many ? 64 * plan->rt : rows;
+  p.tiles = (rows + tile - 1) / tile;
+  p.live_rows = std::min(rows, tile);
+  // Steps of a tile at most: the prefix's, and those from the first token that the window leaves its first query to its last
+  // query's position.
+  const int64_t all = (p.len_cap + 31) / 32, queries = std::min<int64_t>((tile - 1 + p.G - 1) / p.G + 1, p.Q);
+  int64_t steps = all;
+  if (p.window) steps = std::min(all, (p.max_prefix + 31) / 32 + ((int64_t)p.window + queries - 1 + 31) / 32 + 1);
+  const int64_t segments = (int64_t)a->batch * p.Hkv * p.tiles;
+  // Steps of a piece: enough pieces to fill the chip a few times over, so that ragged lengths even out, and not so small that
+  // their merges show.
+  const int64_t target = plan->many ? 2 * bpt::kComputeUnits : 4 * bpt::kComputeUnits;
+  const int64_t least = plan->many ? 8 : 4;
+  int64_t piece = std::max(least, (segments * steps + target - 1) / target);
+  piece = (piece + 3) / 4 * 4;
+  p.piece = (int)std::min<int64_t>(piece, 1 << 26);
+  p.max_pieces = (int)std::max<int64_t>(1, (steps + p.piece - 1) / p.piece);
+  const int64_t slots = segments * p.max_pieces;
+  if (slots > 0x7fffffffLL) return fail(BPT_ERR_INVALID_ARGUMENT, "%s: batch x heads x rows too large", fn);
+  plan->grid = (int)slots;
+  plan->ws_out_floats = p.max_pieces > 1 ? (size_t)slots * p.live_rows * a->head_dim : 0;
+  plan->workspace = p.max_pieces > 1 ? align256((plan->ws_out_floats + (size_t)slots * p.live_rows) * sizeof(float)) : 0;
+  plan->counters = p.max_pieces > 1 ? align256((size_t)segments * sizeof(unsigned)) : 0;
+  *out = p;
+  return BPT_OK;
+}
+
+}  // namespace
+
+int bpt_masked_plan(const bpt_decode_args* a, const bpt_mask_args* m, size_t* workspace_bytes, size_t* counters_bytes) {
+  bpt::MaskedParams p;
+  MaskedPlan plan;
+  int rc = masked_setup(a, m, "bpt_masked_plan", &p, &plan);
+  if (rc) return rc;
+  if (workspace_bytes) *workspace_bytes = plan.workspace;
+  if (counters_bytes) *counters_bytes = plan.counters;
+  return BPT_OK;
+}
+
+int bpt_paged_masked(const bpt_decode_args* a, const bpt_mask_args* m, void* stream) {
+  const char* fn = "bpt_paged_masked";
+  bpt::MaskedParams p;
+  MaskedPlan plan;
+  int rc = masked_setup(a, m, fn, &p, &plan);
+  if (rc || a->batch == 0) return rc;
+  if (!a->q || !a->k_cache || !a->v_cache || !a->block_table || !a->out)
+    return fail(BPT_ERR_INVALID_ARGUMENT, "%s: q, caches, block_table and out must be non-NULL", fn);
+  if (a->kv_dtype != BPT_KV_BF16 && (!a->k_scale || !a->v_scale))
+    return fail(BPT_ERR_INVALID_ARGUMENT, "%s: k_scale and v_scale are required for a quantized cache", fn);
+  const int eb = a->kv_dtype == BPT_KV_BF16 ? 2 : 1;
+  if (!aligned16(a->k_cache) || !aligned16(a->v_cache) || (a->kv_stride_block * eb) % 16 ||
+      (a->kv_stride_token * eb) % 16 || (a->kv_stride_head * eb) % 16)
+    return fail(BPT_ERR_INVALID_ARGUMENT, "%s: cache pointers and strides must be 16-byte aligned", fn);
+  if (!aligned_to(a->q, a->q_stride_b, a->q_stride_q, a->q_stride_h, 2))
+    return fail(BPT_ERR_INVALID_ARGUMENT, "%s: q rows must be 16-byte aligned (pointer and strides)", fn);
+  if (plan.workspace && (!a->workspace || a->workspace_bytes < plan.workspace || ((uintptr_t)a->workspace & 255u)))
+    return fail(BPT_ERR_INVALID_ARGUMENT, "%s: a 256-byte aligned workspace of %zu bytes is required (got %zu)", fn,
+                plan.workspace, a->workspace_bytes);
+  if (plan.counters && (!a->counters || a->counters_bytes < plan.counters || ((uintptr_t)a->counters & 3u)))
+    return fail(BPT_ERR_INVALID_ARGUMENT, "%s: a zeroed counter buffer of %zu bytes is required (got %zu)", fn,
+                plan.counters, a->counters_bytes);
+  p.q = a->q;
+  p.q_sb = a->q_stride_b;
+  p.q_sq = a->q_stride_q;
+  p.q_sh = a->q_stride_h;
+  p.k = (const uint8_t*)a->k_cache;
+  p.v = (const uint8_t*)a->v_cache;
+  p.kv_sblk = a->kv_stride_block * eb;
+  p.kv_stok = a->kv_stride_token * eb;
+  p.kv_shead = a->kv_stride_head * eb;
+  p.ks = a->k_scale;
+  p.vs = a->v_scale;
+  p.sc_sblk = a->scale_stride_block;
+  p.sc_stok = a->scale_stride_token;
+  p.sc_shead = a->scale_stride_head;
+  p.table = a->block_table;
+  p.table_sb = a->table_stride_b;
+  p.table_i64 = a->table_dtype == BPT_IDX_I64;
+  p.lens = a->context_lens;
+  p.out = a->out;
+  p.o_sb = a->out_stride_b;
+  p.o_sq = a->out_stride_q;
+  p.o_sh = a->out_stride_h;
+  p.out_dtype = a->out_dtype;
+  p.lse_out = a->lse_out;
+  p.slopes = m->slopes;
+  p.prefix_lens = m->prefix_lens;
+  p.starts = m->starts;
+  p.st_sb = m->start_stride_b;
+  p.st_sq = m->start_stride_q;
+  p.ws_out = (float*)a->workspace;
+  p.ws_lse = p.ws_out + plan.ws_out_floats;
+  p.counters = (unsigned*)a->counters;
+  const bool split = a->q_dtype == BPT_F_F16;
+  const bool head = a->scale_kind == BPT_SCALE_PER_HEAD;
+  auto launch = a->kv_dtype == BPT_KV_BF16 ? bpt::launch_masked_bf16
+                : a->kv_dtype == BPT_KV_FP8_E4M3FN ? (head ? bpt::launch_masked_fp8_head : bpt::launch_masked_fp8_token)
+                                                   : (head ? bpt::launch_masked_int8_head : bpt::launch_masked_int8_token);
+  hipError_t e = launch(p, split, plan.rt, plan.many, plan.grid, (hipStream_t)stream);
+  if (e != hipSuccess) return hip_fail(fn, e);
+  return BPT_OK;
+}
+
+namespace {
+
 // Whether rows of `elem`-byte channels can be loaded 8 at a time.
 bool rows_aligned(const void* p, int64_t sb, int64_t sq, int64_t sh, int elem) {
   return !p || aligned_to(p, sb, sq, sh, elem);

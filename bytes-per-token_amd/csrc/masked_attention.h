@@ -1,0 +1,891 @@
+// Paged attention with masked and shaped scores: scores capped by a tanh, a bias that falls with distance, a sliding
+// window, a prefix that every query of a sequence sees, and a first token per query (documents packed into a sequence).
+//
+// Row r = (query i, head h G + g) of KV head h sits at position p = len - Q + i. It sees token j of its sequence when
+//   j < len  and  (j < prefix  or  (max(start_i, p - window + 1) <= j <= p)),
+// and with t = sm_scale q.k its score is t, or cap tanh(t / cap), less slope_h |p - j|. Scores are held in float32 in units
+// of log2 e, so that weights are 2^(score - max); with E = 2^(2 log2e t / cap) the cap is A - 2 A / (1 + E), A = cap log2e.
+// That form loses about A 2^-23 absolutely, 7e-5 of a weight at the largest cap that uses it (kMaskedPlainCap); beyond, small
+// arguments take tanh's series.
+//
+// Products run on the matrix cores in bf16, transposed: S^T (16 tokens x 16 rows) = K Q^T, O^T (16 channels x 16 rows) +=
+// V^T P^T. All three formats' codes are exact in bf16 (8 significant bits); an f16 q is split into two bf16 parts (exact) and
+// the weights into two (16 bits: a weight's error is 2^-17, under the 2^-12 of an f16 output's half step). In the
+// 16x16x32 layout a lane holds row n = lane % 16 and, with g = lane / 16, the scores of tokens 4 g + i and 16 + 4 g + i of 32;
+// they are taken as elements 8 g + e of the second product's contraction, so weights never leave their lane. A V operand
+// then needs 8 tokens of one channel per lane: a lane loads 8 channels (8 lane % 16 ..) of its 8 tokens, whole rows by 16
+// lanes, and transposes them in registers. Output channel 8 (4 g + i) + c of row n is element i of O^T's block c.
+//
+// Work is cut into steps of 32 tokens; a tile (rows of one (sequence, KV head)) lists the steps that some row of it sees:
+// those of the prefix, then those from its lowest first token to its last position. Steps are dealt out in pieces of a fixed
+// number of steps, one per workgroup: ragged batches balance by themselves, and windows cost no launch over the tokens
+// before them. The pieces of a tile meet in float32 partials, which the last workgroup to arrive combines in order.
+//
+// Two kernels:
+//  * few rows (up to 32 of a KV head): the waves of a workgroup take steps in turn, straight from memory into registers,
+//    and merge through LDS at the end. Bound by the cache's bytes.
+//  * many rows: a workgroup's four waves hold 64 or 128 rows; each of two steps' keys and values is loaded and converted by
+//    one wave and read by all from LDS, where operands lie in the order lanes take them (no bank conflicts, no swizzle).
+//    Bound by the vector units (the scores' exponentials).
+//
+// Tokens a row does not see must add nothing to it, but 0 times an infinity is a NaN: a wave whose result is not finite does
+// its piece again with values that are not finite taken out of the products and added one by one to the rows that see them.
+// Finite data pays one look at the result.
+#pragma once
+
+#include "decode_common.h"
+
+namespace bpt {
+
+typedef __bf16 mbf16x8 __attribute__((ext_vector_type(8)));
+typedef float mf32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t mu32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t mu32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int kMaskedStep = 32;
+constexpr float kMaskedSlack = 8.0f;  // a row's reference point may lag its maximum by this (log2): weights stay below 2^8
+
+// ---- conversions ------------------------------------------------------------------------------------------------
+
+__device__ __forceinline__ uint32_t masked_fp8_pair(uint32_t w, bool high) {
+  return high ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, true))
+              : __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, false));
+}
+// Four int8 codes -> bf16, through float32 (exact).
+__device__ __forceinline__ mu32x2 masked_int8x4(uint32_t w) {
+  const uint32_t u = w ^ 0x80808080u;
+  float f[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) f[i] = (float)((u >> (8 * i)) & 0xffu) - 128.0f;
+  return mu32x2{__builtin_amdgcn_perm(__float_as_uint(f[1]), __float_as_uint(f[0]), 0x07060302u),
+                __builtin_amdgcn_perm(__float_as_uint(f[3]), __float_as_uint(f[2]), 0x07060302u)};
+}
+// Eight codes (two dwords) -> bf16.
+template <int KV>
+__device__ __forceinline__ mu32x4 masked_codes8(uint32_t w0, uint32_t w1) {
+  if constexpr (KV == kKvFp8) {
+    return mu32x4{masked_fp8_pair(w0, false), masked_fp8_pair(w0, true), masked_fp8_pair(w1, false), masked_fp8_pair(w1, true)};
+  } else {
+    const mu32x2 a = masked_int8x4(w0), b = masked_int8x4(w1);
+    return mu32x4{a.x, a.y, b.x, b.y};
+  }
+}
+// 4 x 4 byte transpose: w[i] byte j -> out[j] byte i.
+__device__ __forceinline__ void masked_transpose4(uint32_t w0, uint32_t w1, uint32_t w2, uint32_t w3, uint32_t* o) {
+  const uint32_t t0 = __builtin_amdgcn_perm(w1, w0, 0x05010400u), t1 = __builtin_amdgcn_perm(w3, w2, 0x05010400u);
+  const uint32_t t2 = __builtin_amdgcn_perm(w1, w0, 0x07030602u), t3 = __builtin_amdgcn_perm(w3, w2, 0x07030602u);
+  o[0] = __builtin_amdgcn_perm(t1, t0, 0x05040100u);
+  o[1] = __builtin_amdgcn_perm(t1, t0, 0x07060302u);
+  o[2] = __builtin_amdgcn_perm(t3, t2, 0x05040100u);
+  o[3] = __builtin_amdgcn_perm(t3, t2, 0x07060302u);
+}
+// Two bf16 values with those that are not finite replaced by zeros.
+__device__ __forceinline__ uint32_t masked_finite2(uint32_t x) {
+  if ((x & 0x7f80u) == 0x7f80u) x &= 0xffff0000u;
+  if ((x & 0x7f800000u) == 0x7f800000u) x &= 0xffffu;
+  return x;
+}
+__device__ __forceinline__ mf32x4 masked_mfma(mu32x4 a, mu32x4 b, mf32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(mbf16x8, a), __builtin_bit_cast(mbf16x8, b), c, 0, 0, 0);
+}
+
+// ---- one step's codes -------------------------------------------------------------------------------------------
+
+template <int KV>
+struct MaskedRaw {
+  static constexpr int kWords = KV == kKvBf16 ? 32 : 16;
+  uint32_t w[kWords];
+};
+
+// The pages (clamped into the pool) of a step's two 16-token groups, for page sizes of at least 16.
+struct MaskedPages {
+  int e[2];
+};
+__device__ __forceinline__ int masked_clamp_page(const MaskedParams& p, int e) {
+  return e < 0 ? 0 : (e >= p.num_blocks ? p.num_blocks - 1 : e);
+}
+__device__ __forceinline__ MaskedPages masked_pages(const MaskedParams& p, int b, int token0, int len) {
+  MaskedPages g{{0, 0}};
+  if (p.logP >= 4) {
+    const int32_t* table = (const int32_t*)p.table;
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+      g.e[t] = load_uniform(table + (((int64_t)b * p.table_sb + (min(token0 + 16 * t, len - 1) >> p.logP)) << p.table_i64));
+  }
+  return g;
+}
+// Byte offset of a token's row of head h in the pools (any page size). Tokens past the last one read it instead.
+__device__ __forceinline__ int64_t masked_row(const MaskedParams& p, int b, int h, int token, int len) {
+  const int tok = min(token, len - 1);
+  const int e = masked_clamp_page(p, ((const int32_t*)p.table)[((int64_t)b * p.table_sb + (tok >> p.logP)) << p.table_i64]);
+  return (int64_t)e * p.kv_sblk + (int64_t)(tok & (p.P - 1)) * p.kv_stok + (int64_t)h * p.kv_shead;
+}
+// The 16-token group's base offset and the last of its rows that may be read.
+__device__ __forceinline__ int64_t masked_group(const MaskedParams& p, int h, int e, int token, int len, int& rmax) {
+  rmax = max(len - 1 - token, 0);
+  return (int64_t)masked_clamp_page(p, sread(e)) * p.kv_sblk + (int64_t)(min(token, len - 1) & (p.P - 1)) * p.kv_stok +
+         (int64_t)h * p.kv_shead;
+}
+
+// ONCE: read by this workgroup alone (past the caches), else by the other tiles of the head too.
+template <int W, bool ONCE>
+__device__ __forceinline__ void masked_load(const uint8_t* src, uint32_t* w) {
+  typedef uint32_t words __attribute__((ext_vector_type(W)));
+  const words x = ONCE ? __builtin_nontemporal_load((const words*)src) : *(const words*)src;
+#pragma unroll
+  for (int i = 0; i < W; ++i) w[i] = x[i];
+}
+
+// Keys: lane (n, g) takes token n of both 16-token groups; of bf16 channels 32 s + 8 g .. + 7 for product s, of codes
+// 64 j + 16 g .. + 15 for products 2 j and 2 j + 1.
+template <int KV, bool ONCE>
+__device__ __forceinline__ void masked_issue_k(const MaskedParams& p, int b, int h, int token0, int len, MaskedPages pages,
+                                               int lane, MaskedRaw<KV>& r) {
+  constexpr int KL = KV == kKvBf16 ? 4 : 2;
+  const int n = lane & 15, g = lane >> 4;
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    const uint8_t* src;
+    if (p.logP >= 4) {
+      int rmax;
+      const int64_t base = masked_group(p, h, pages.e[t], token0 + 16 * t, len, rmax);
+      src = p.k + base + (uint32_t)(min(n, rmax) * (uint32_t)p.kv_stok + 16 * g);
+    } else {
+      src = p.k + masked_row(p, b, h, token0 + 16 * t + n, len) + 16 * g;
+    }
+#pragma unroll
+    for (int j = 0; j < KL; ++j) masked_load<4, ONCE>(src + 64 * j, r.w + 4 * (KL * t + j));
+  }
+}
+// Values: lane (n, g) takes channels 8 n .. + 7 of tokens 4 g + i and 16 + 4 g + i.
+template <int KV, bool ONCE>
+__device__ __forceinline__ void masked_issue_v(const MaskedParams& p, int b, int h, int token0, int len, MaskedPages pages,
+                                               int lane, MaskedRaw<KV>& r) {
+  constexpr int W = KV == kKvBf16 ? 4 : 2;
+  const int n = lane & 15, g = lane >> 4;
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    int rmax = 0;
+    const int64_t base = p.logP >= 4 ? masked_group(p, h, pages.e[t], token0 + 16 * t, len, rmax) : 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint8_t* src = p.logP >= 4 ? p.v + base + (uint32_t)(min(4 * g + i, rmax) * (uint32_t)p.kv_stok + 4 * W * n)
+                                       : p.v + masked_row(p, b, h, token0 + 16 * t + 4 * g + i, len) + 4 * W * n;
+      masked_load<W, ONCE>(src, r.w + W * (4 * t + i));
+    }
+  }
+}
+// Per-token scales: lane l < 32 takes the key's scale of token l, the others the value's of token l - 32.
+__device__ __forceinline__ float masked_issue_scale(const MaskedParams& p, int b, int h, int token0, int len, MaskedPages pages,
+                                                    int lane) {
+  const int tok = min(token0 + (lane & 31), len - 1);
+  int e;
+  if (p.logP >= 4) e = (lane & 16) ? pages.e[1] : pages.e[0];
+  else e = ((const int32_t*)p.table)[((int64_t)b * p.table_sb + (tok >> p.logP)) << p.table_i64];
+  return (lane < 32 ? p.ks : p.vs)[(int64_t)masked_clamp_page(p, e) * p.sc_sblk + (int64_t)(tok & (p.P - 1)) * p.sc_stok +
+                                   (int64_t)h * p.sc_shead];
+}
+
+// The key operand of product s over 16-token group t.
+template <int KV>
+__device__ __forceinline__ mu32x4 masked_k_frag(const MaskedRaw<KV>& r, int t, int s) {
+  if constexpr (KV == kKvBf16) {
+    const uint32_t* w = r.w + 4 * (4 * t + s);
+    return mu32x4{w[0], w[1], w[2], w[3]};
+  } else {
+    const uint32_t* w = r.w + 4 * (2 * t + (s >> 1)) + 2 * (s & 1);
+    return masked_codes8<KV>(w[0], w[1]);
+  }
+}
+// The value operands of four channel blocks c = 4 q .. 4 q + 3: channel 8 n + c of the lane's 8 tokens. CAREFUL: with values
+// that are not finite replaced by zeros.
+template <int KV, bool CAREFUL>
+__device__ __forceinline__ void masked_v_frags(const MaskedRaw<KV>& r, int q, mu32x4 (&f)[4]) {
+  if constexpr (KV == kKvBf16) {
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const uint32_t sel = (c & 1) ? 0x07060302u : 0x05040100u;
+      const int d = 2 * q + (c >> 1);  // the dword of a token's channels that holds channel 4 q + c
+#pragma unroll
+      for (int e = 0; e < 4; ++e) f[c][e] = __builtin_amdgcn_perm(r.w[4 * (2 * e + 1) + d], r.w[4 * (2 * e) + d], sel);
+    }
+  } else {
+    uint32_t lo[4], hi[4];
+    masked_transpose4(r.w[q], r.w[2 + q], r.w[4 + q], r.w[6 + q], lo);
+    masked_transpose4(r.w[8 + q], r.w[10 + q], r.w[12 + q], r.w[14 + q], hi);
+#pragma unroll
+    for (int c = 0; c < 4; ++c) f[c] = masked_codes8<KV>(lo[c], hi[c]);
+  }
+  if constexpr (CAREFUL && KV != kKvInt8) {
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) f[c][e] = masked_finite2(f[c][e]);
+  }
+}
+
+// ---- rows -------------------------------------------------------------------------------------------------------
+
+// What one lane knows of row n of each of its RT row tiles.
+template <int RT>
+struct MaskedRows {
+  int pos[RT];         // the row's position
+  int lo[RT], hi[RT];  // tokens lo .. hi - 1 are seen behind the prefix
+  float slope[RT];     // times log2 e
+  float m[RT], l[RT];  // reference point, and this lane's share of the weights' sum
+  mf32x4 o[RT][8];     // channels 8 (4 g + i) + c of block c
+};
+
+// The steps of a tile, and which of them all of its rows see whole.
+struct MaskedRange {
+  int len, prefix;
+  int sa, sb, n;        // steps 0 .. sa - 1, then sb ..; n in all
+  int max_lo, min_hi;   // every row sees tokens max_lo .. min_hi - 1
+  int min_lo, max_hi;   // some row sees tokens min_lo .. max_hi - 1 behind the prefix
+};
+__device__ __forceinline__ int masked_token0(const MaskedRange& r, int t) { return kMaskedStep * (t < r.sa ? t : r.sb + t - r.sa); }
+
+__device__ __forceinline__ void masked_bounds(const MaskedParams& p, int b, int qi, int len, int& pos, int& lo, int& hi) {
+  pos = len - p.Q + qi;
+  lo = p.window > 0 ? max(pos - p.window + 1, 0) : 0;
+  if (p.starts) lo = max(lo, p.starts[(int64_t)b * p.st_sb + (int64_t)qi * p.st_sq]);
+  hi = min(pos + 1, len);
+  if (hi <= lo) hi = lo = 0;  // nothing behind the prefix
+}
+
+// Lowest / highest bounds over rows r0 .. r1 - 1 of a KV head, the same in every lane.
+__device__ __forceinline__ void masked_extent(const MaskedParams& p, int b, int r0, int r1, int lane, MaskedRange& r) {
+  r.min_lo = 0x7fffffff, r.max_lo = 0, r.min_hi = 0x7fffffff, r.max_hi = 0;
+  const int q0 = r0 / p.G, q1 = (r1 - 1) / p.G;
+  int pos, lo, hi;
+  const bool scan = p.starts != nullptr;  // else both bounds rise with the query: the first and the last one tell
+  for (int q = scan ? q0 + lane : q0; q <= q1; q += scan ? 64 : max(q1 - q0, 1)) {
+    masked_bounds(p, b, q, r.len, pos, lo, hi);
+    r.max_lo = max(r.max_lo, lo), r.min_hi = min(r.min_hi, hi), r.max_hi = max(r.max_hi, hi);
+    if (hi > lo) r.min_lo = min(r.min_lo, lo);
+    else if (!scan) r.min_lo = 0;  // positions below 0: the first row that sees anything sees token 0
+  }
+  if (scan) {
+#pragma unroll
+    for (int m = 32; m >= 1; m >>= 1) {
+      r.min_lo = min(r.min_lo, __shfl_xor(r.min_lo, m, 64)), r.max_lo = max(r.max_lo, __shfl_xor(r.max_lo, m, 64));
+      r.min_hi = min(r.min_hi, __shfl_xor(r.min_hi, m, 64)), r.max_hi = max(r.max_hi, __shfl_xor(r.max_hi, m, 64));
+    }
+  }
+  r.min_lo = sread(r.min_lo), r.max_lo = sread(r.max_lo), r.min_hi = sread(r.min_hi), r.max_hi = sread(r.max_hi);
+}
+// The sequence's length and prefix, and the tile's steps.
+__device__ __forceinline__ MaskedRange masked_range(const MaskedParams& p, int b, int r0, int r1, int lane) {
+  MaskedRange r;
+  int len = p.lens ? load_uniform(p.lens + b) : p.len_cap;
+  r.len = min(max(len, 0), p.len_cap);
+  r.prefix = p.prefix_lens ? min(min(max(load_uniform(p.prefix_lens + b), 0), p.max_prefix), r.len) : 0;
+  masked_extent(p, b, r0, r1, lane, r);
+  r.sa = (r.prefix + kMaskedStep - 1) / kMaskedStep;
+  r.sb = r.sa;
+  r.n = r.sa;
+  if (r.max_hi > 0) {
+    r.sb = max(r.min_lo / kMaskedStep, r.sa);
+    r.n = r.sa + max((r.max_hi + kMaskedStep - 1) / kMaskedStep - r.sb, 0);
+  }
+  return r;
+}
+__device__ __forceinline__ bool masked_whole(const MaskedRange& r, int token0) {
+  const int end = token0 + kMaskedStep;
+  return end <= r.prefix || (token0 >= r.max_lo && end <= r.min_hi);
+}
+__device__ __forceinline__ bool masked_unseen(const MaskedRange& r, int token0) {
+  return token0 >= r.prefix && (token0 >= r.max_hi || token0 + kMaskedStep <= r.min_lo);
+}
+
+template <int RT>
+__device__ __forceinline__ void masked_rows_init(const MaskedParams& p, int b, int h, int first, int rows, int len, int lane,
+                                                 MaskedRows<RT>& s) {
+#pragma unroll
+  for (int t = 0; t < RT; ++t) {
+    const int r = min(first + 16 * t + (lane & 15), rows - 1);  // lanes past the last row repeat it
+    const int qi = r / p.G;
+    masked_bounds(p, b, qi, len, s.pos[t], s.lo[t], s.hi[t]);
+    s.slope[t] = p.slopes ? p.slopes[h * p.G + r - qi * p.G] * kLog2e : 0.0f;
+  }
+}
+template <int RT>
+__device__ __forceinline__ void masked_rows_reset(MaskedRows<RT>& s) {
+#pragma unroll
+  for (int t = 0; t < RT; ++t) {
+    s.m[t] = kNegInf, s.l[t] = 0.0f;
+#pragma unroll
+    for (int c = 0; c < 8; ++c) s.o[t][c] = mf32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  }
+}
+
+// Queries as the first product's B operands: q[rt][s], and with an f16 q the remainders behind them.
+template <int KV, bool QS, int RT>
+__device__ __forceinline__ void masked_load_q(const MaskedParams& p, int b, int h, int first, int rows, int lane,
+                                              mu32x4 (&q)[RT][QS ? 8 : 4]) {
+  const int g = lane >> 4;
+#pragma unroll
+  for (int t = 0; t < RT; ++t) {
+    const int r = min(first + 16 * t + (lane & 15), rows - 1);
+    const int qi = r / p.G;
+    const uint16_t* src = (const uint16_t*)p.q + (int64_t)b * p.q_sb + (int64_t)qi * p.q_sq + (int64_t)(h * p.G + r - qi * p.G) * p.q_sh;
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      const int c = KV == kKvBf16 ? 32 * s + 8 * g : 64 * (s >> 1) + 16 * g + 8 * (s & 1);
+      const mu32x4 w = *(const mu32x4*)(src + c);
+      if constexpr (!QS) {
+        q[t][s] = w;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float x0 = (float)__builtin_bit_cast(_Float16, (uint16_t)(w[e] & 0xffffu));
+          const float x1 = (float)__builtin_bit_cast(_Float16, (uint16_t)(w[e] >> 16));
+          const bf16x2 hi = pack_bf16(x0, x1);
+          q[t][s][e] = __builtin_bit_cast(uint32_t, hi);
+          q[t][4 + s][e] = __builtin_bit_cast(uint32_t, pack_bf16(x0 - (float)hi[0], x1 - (float)hi[1]));
+        }
+      }
+    }
+  }
+}
+
+// Values that are not finite, of the step's tokens, added to the row's outputs where it sees them (weights: each token's
+// weight before its value's scale, at weights[16 token + n], -1 for tokens that row n does not see).
+template <int KV, int SK>
+__device__ __forceinline__ void masked_add_nonfinite(const MaskedParams& p, int b, int h, int token0, int len, int lane,
+                                                     const float* weights, mf32x4 (&o)[8]) {
+  const int n = lane & 15, g = lane >> 4;
+  for (int j = 0; j < kMaskedStep; ++j) {
+    const int tok = min(token0 + j, len - 1);
+    const uint8_t* src = p.v + masked_row(p, b, h, tok, len);
+    float vs = 1.0f;
+    if constexpr (SK == kScaleTokenHead) {
+      const int e = masked_clamp_page(p, ((const int32_t*)p.table)[((int64_t)b * p.table_sb + (tok >> p.logP)) << p.table_i64]);
+      vs = p.vs[(int64_t)e * p.sc_sblk + (int64_t)(tok & (p.P - 1)) * p.sc_stok + (int64_t)h * p.sc_shead];
+    }
+    const bool scale_bad = !(fabsf(vs) <= __FLT_MAX__);
+    const float w = weights[16 * j + n];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
+        const int ch = 32 * g + 8 * i + c;
+        float v;
+        if constexpr (KV == kKvBf16) {
+          v = bf16_bits_to_f32(((const uint16_t*)src)[ch]);
+        } else if constexpr (KV == kKvFp8) {
+          float f[4];
+          fp8x4_to_f32(src[ch], f);
+          v = f[0];
+        } else {
+          v = (float)(int8_t)src[ch];
+        }
+        if ((scale_bad || !(fabsf(v) <= __FLT_MAX__)) && w >= 0.0f) o[c][i] += w * (v * vs);
+      }
+  }
+}
+
+// Scores S[rt][t] (token 16 t + 4 g + i, raw products) -> weights' two bf16 parts w[rt][part], the rows' state brought up to
+// date. sc: per-token scales of the step (keys' 32, then values' 32). careful (uniform): values that are not finite stay out of
+// the products and are added here instead (weights: this wave's 512 floats of LDS for that).
+template <int KV, int SK, int RT, bool CAREFUL>
+__device__ __forceinline__ void masked_softmax(const MaskedParams& p, const MaskedRange& rg, int b, int h, int token0, bool whole,
+                                               int lane, float qs, const float* sc, mf32x4 (&S)[RT][2], MaskedRows<RT>& st,
+                                               mu32x4 (&w)[RT][2], float* weights) {
+  const int n = lane & 15, g = lane >> 4;
+  float kf[8], vf[8];
+  if constexpr (SK == kScaleTokenHead) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        kf[4 * t + i] = sc[16 * t + 4 * g + i] * qs;
+        vf[4 * t + i] = sc[32 + 16 * t + 4 * g + i];
+      }
+  }
+#pragma unroll
+  for (int r = 0; r < RT; ++r) {
+    float x[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = S[r][e >> 2][e & 3] * (SK == kScaleTokenHead ? kf[e] : qs);
+    if (p.cap > 0.0f) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float u = x[e];  // 2 log2e t / cap
+        const float y = p.cap - 2.0f * p.cap * __builtin_amdgcn_rcpf(1.0f + fast_exp2(u));
+        x[e] = y;
+        if (p.cap > kMaskedPlainCap) {  // tanh z = z (1 - z^2 / 3 + 2 z^4 / 15 - 17 z^6 / 315), z = u ln2 / 2
+          const float z = u * (0.5f * kLn2), z2 = z * z;
+          const float series = fmaf(z2, fmaf(z2, fmaf(z2, -17.0f / 315.0f, 2.0f / 15.0f), -1.0f / 3.0f), 1.0f);
+          if (fabsf(z) < 0.25f) x[e] = p.cap * z * series;
+        }
+      }
+    }
+    if (p.slopes) {
+      const float d0 = (float)(st.pos[r] - token0 - 4 * g);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = fmaf(-st.slope[r], fabsf(d0 - (float)(16 * (e >> 2) + (e & 3))), x[e]);
+    }
+    uint32_t seen = 0xffu;
+    if (!whole) {
+      seen = 0u;
+      const int j0 = token0 + 4 * g;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int j = j0 + 16 * (e >> 2) + (e & 3);
+        const bool s = j < rg.prefix || (unsigned)(j - st.lo[r]) < (unsigned)(st.hi[r] - st.lo[r]);
+        seen |= s ? 1u << e : 0u;
+        x[e] = s ? x[e] : kNegInf;
+      }
+    }
+    float mx = x[0];
+#pragma unroll
+    for (int e = 1; e < 8; ++e) mx = fmaxf(mx, x[e]);
+    mx = max_xor<32>(max_xor<16>(mx));
+    if (__any(mx > st.m[r] + kMaskedSlack)) {  // some row's maximum left its reference point behind
+      const float m = fmaxf(st.m[r], mx);
+      const float a = st.m[r] == kNegInf ? 0.0f : fast_exp2(st.m[r] - m);
+      st.m[r] = m;
+      st.l[r] *= a;
+#pragma unroll
+      for (int c = 0; c < 8; ++c) st.o[r][c] *= a;
+    }
+    const float m = st.m[r] == kNegInf ? 0.0f : st.m[r];
+    float sum = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      x[e] = fast_exp2(x[e] - m);
+      sum += x[e];
+    }
+    st.l[r] += sum;
+    if constexpr (CAREFUL) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        weights[(16 * (e >> 2) + 4 * g + (e & 3)) * 16 + n] = (seen >> e) & 1u ? x[e] : -1.0f;
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // the wave's lanes read one another's
+      masked_add_nonfinite<KV, SK>(p, b, h, token0, rg.len, lane, weights, st.o[r]);
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    }
+    if constexpr (SK == kScaleTokenHead) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        x[e] *= vf[e];
+        if (!whole && !((seen >> e) & 1u)) x[e] = 0.0f;  // an unseen token's scale may be anything
+        if (CAREFUL && !(fabsf(vf[e]) <= __FLT_MAX__)) x[e] = 0.0f;
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const bf16x2 hi = pack_bf16(x[2 * e], x[2 * e + 1]);
+      w[r][0][e] = __builtin_bit_cast(uint32_t, hi);
+      w[r][1][e] = __builtin_bit_cast(uint32_t, pack_bf16(x[2 * e] - (float)hi[0], x[2 * e + 1] - (float)hi[1]));
+    }
+  }
+}
+
+// Whether this lane's sums hold anything that is not finite.
+template <int RT>
+__device__ __forceinline__ bool masked_nonfinite(const MaskedRows<RT>& st) {
+  float z = 0.0f;
+#pragma unroll
+  for (int r = 0; r < RT; ++r)
+#pragma unroll
+    for (int c = 0; c < 8; ++c)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) z = fmaf(st.o[r][c][i], 0.0f, z);
+  return z != 0.0f;
+}
+
+// The multiplier of raw products that gives scores in log2 units, or with a cap the argument of its exponential.
+template <int SK>
+__device__ __forceinline__ float masked_qscale(const MaskedParams& p, int h) {
+  return SK == kScaleHead ? p.qscale * p.ks[h] : p.qscale;
+}
+
+// One output element's row, and a lane's 32 channels of it from `ch` on.
+__device__ __forceinline__ void masked_write(const MaskedParams& p, int b, int h, int r, int ch, int count, const float* o, float lse2) {
+  const int qi = r / p.G, hq = h * p.G + r - qi * p.G;
+  const int64_t at = (int64_t)b * p.o_sb + (int64_t)qi * p.o_sq + (int64_t)hq * p.o_sh + ch;
+  for (int i = 0; i < count; ++i) store_float(p.out, at + i, p.out_dtype, o[i]);
+  if (p.lse_out && ch == 0) p.lse_out[((int64_t)b * p.Q + qi) * p.Hq + hq] = lse2 == kNegInf ? kNegInf : lse2 * kLn2;
+}
+
+// A tile's n pieces (slots slot0 ..) combined by the last of them to arrive, the whole workgroup of NT threads: two channels of
+// a row a thread, the pieces in order, so that the sum does not depend on who came last.
+template <int NT>
+__device__ __forceinline__ void masked_combine(const MaskedParams& p, int b, int h, int r0, int live, int64_t slot0, int n, int tid) {
+  ws_acquire();
+  for (int idx = tid; idx < live * (kHeadDim / 2); idx += NT) {
+    const int row = idx / (kHeadDim / 2), ch = 2 * (idx - row * (kHeadDim / 2));
+    const float* lse = p.ws_lse + slot0 * p.live_rows + row;
+    const float* prt = p.ws_out + (slot0 * p.live_rows + row) * kHeadDim + ch;
+    float M = kNegInf, W = 0.0f, o[2] = {0.0f, 0.0f};
+    for (int j0 = 0; j0 < n; j0 += 8) {
+      float lv[8], ov[8][2], top = kNegInf;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        lv[j] = kNegInf, ov[j][0] = ov[j][1] = 0.0f;
+        if (j0 + j < n) {
+          lv[j] = ws_load(lse + (int64_t)(j0 + j) * p.live_rows);
+          ws_load2(prt + (int64_t)(j0 + j) * p.live_rows * kHeadDim, ov[j][0], ov[j][1]);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) top = fmaxf(top, lv[j]);
+      const float nm = fmaxf(M, top), mu = nm == kNegInf ? 0.0f : nm;
+      const float a = W > 0.0f ? fast_exp2(M - mu) : (W != W ? W : 0.0f);
+      W *= a, o[0] *= a, o[1] *= a;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        if (lv[j] == kNegInf) continue;  // an empty piece
+        const float e = fast_exp2(lv[j] - mu);
+        W += e;
+        o[0] = fmaf(e, ov[j][0], o[0]), o[1] = fmaf(e, ov[j][1], o[1]);
+      }
+      M = nm;
+    }
+    const float inv = W == 0.0f ? 0.0f : 1.0f / W;
+    o[0] *= inv, o[1] *= inv;
+    masked_write(p, b, h, r0 + row, ch, 2, o, W == 0.0f ? kNegInf : M + __log2f(W));
+  }
+}
+
+// A workgroup's place: XCD-major (workgroups go to the 8 XCDs in turn, each with its own L2), so that the heads of a page
+// (few rows) or the tiles of a head (many rows) meet in one L2.
+__device__ __forceinline__ int masked_index() {
+  const int x = blockIdx.x, n = gridDim.x;
+  const int q = n >> 3, r = n & 7, k = x & 7;
+  return k * q + min(k, r) + (x >> 3);
+}
+
+// ---- few rows ---------------------------------------------------------------------------------------------------
+
+constexpr int kMaskedRowPad = kHeadDim + 4;  // floats of a row in LDS: 16 rows spread over the banks
+
+// One wave's steps t0 + wave, t0 + wave + 4, ... < t1 folded into its rows. The next step's codes are requested as soon as the
+// registers of this one's are free.
+template <int KV, int SK, bool QS, int RT, bool CAREFUL>
+__device__ __forceinline__ void masked_few_steps(const MaskedParams& p, const MaskedRange& rg, int b, int h, int t, int t1, int lane,
+                                                 float qs, const mu32x4 (&q)[RT][QS ? 8 : 4], float* w_scale, float* w_weights,
+                                                 MaskedRows<RT>& st) {
+  masked_rows_reset(st);
+  if (t >= t1) return;
+  MaskedRaw<KV> k, vv;
+  float sc = 0.0f;
+  int token0 = masked_token0(rg, t);
+  MaskedPages pages = masked_pages(p, b, token0, rg.len);
+  masked_issue_k<KV, true>(p, b, h, token0, rg.len, pages, lane, k);
+  masked_issue_v<KV, true>(p, b, h, token0, rg.len, pages, lane, vv);
+  if constexpr (SK == kScaleTokenHead) sc = masked_issue_scale(p, b, h, token0, rg.len, pages, lane);
+  pages = masked_pages(p, b, masked_token0(rg, min(t + 4, t1 - 1)), rg.len);
+  for (; t < t1; t += 4) {
+    mf32x4 S[RT][2];
+#pragma unroll
+    for (int r = 0; r < RT; ++r) S[r][0] = S[r][1] = mf32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+        const mu32x4 f = masked_k_frag<KV>(k, u, s);
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+          if constexpr (QS) S[r][u] = masked_mfma(f, q[r][4 + s], S[r][u]);
+          S[r][u] = masked_mfma(f, q[r][s], S[r][u]);
+        }
+      }
+    const int next = masked_token0(rg, min(t + 4, t1 - 1));
+    if (t + 4 < t1) masked_issue_k<KV, true>(p, b, h, next, rg.len, pages, lane, k);
+    if constexpr (SK == kScaleTokenHead) {
+      w_scale[lane] = sc;
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      if (t + 4 < t1) sc = masked_issue_scale(p, b, h, next, rg.len, pages, lane);
+    }
+    mu32x4 w[RT][2];
+    masked_softmax<KV, SK, RT, CAREFUL>(p, rg, b, h, token0, masked_whole(rg, token0), lane, qs, w_scale, S, st, w, w_weights);
+#pragma unroll
+    for (int c4 = 0; c4 < 2; ++c4) {
+      mu32x4 f[4];
+      masked_v_frags<KV, CAREFUL>(vv, c4, f);
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+          st.o[r][4 * c4 + c] = masked_mfma(f[c], w[r][1], st.o[r][4 * c4 + c]);
+          st.o[r][4 * c4 + c] = masked_mfma(f[c], w[r][0], st.o[r][4 * c4 + c]);
+        }
+    }
+    if (t + 4 < t1) masked_issue_v<KV, true>(p, b, h, next, rg.len, pages, lane, vv);
+    pages = masked_pages(p, b, masked_token0(rg, min(t + 8, t1 - 1)), rg.len);
+    token0 = next;
+  }
+}
+
+template <int KV, int SK, bool QS, int RT>
+__global__ __launch_bounds__(256, RT == 1 ? 3 : 2) void masked_few_kernel(const MaskedParams p) {
+  extern __shared__ float smem[];  // [4 waves][live][kMaskedRowPad], then [4 waves][live] m and l; scales and weights on the way
+  __shared__ int s_last;
+  const int tid = threadIdx.x, lane = tid & 63, wave = sread(tid >> 6);
+  const int n = lane & 15, g = lane >> 4;
+  int v = masked_index();
+  const int h = v % p.Hkv;
+  v /= p.Hkv;
+  const int piece = v % p.max_pieces, b = v / p.max_pieces;
+  const int rows = p.Q * p.G;
+  const MaskedRange rg = masked_range(p, b, 0, rows, lane);
+  const int pieces = max((rg.n + p.piece - 1) / p.piece, 1);
+  if (piece >= pieces) return;
+  const int t0 = piece * p.piece, t1 = min(t0 + p.piece, rg.n);
+  const int live = rows;
+
+  MaskedRows<RT> st;
+  masked_rows_init<RT>(p, b, h, 0, rows, rg.len, lane, st);
+  mu32x4 q[RT][QS ? 8 : 4];
+  masked_load_q<KV, QS, RT>(p, b, h, 0, rows, lane, q);
+  const float qs = masked_qscale<SK>(p, h);
+  float* w_scale = smem + wave * 64;                             // this wave's per-token scales
+  float* w_weights = smem + 4 * 64 + wave * kMaskedStep * 16;  // and, where needed, its weights
+
+  masked_few_steps<KV, SK, QS, RT, false>(p, rg, b, h, t0 + wave, t1, lane, qs, q, w_scale, w_weights, st);
+  if (__any(masked_nonfinite(st)))
+    masked_few_steps<KV, SK, QS, RT, true>(p, rg, b, h, t0 + wave, t1, lane, qs, q, w_scale, w_weights, st);
+
+  // The waves' shares of each row, brought to the row's maximum and added.
+  float* s_o = smem;
+  float* s_m = smem + 4 * live * kMaskedRowPad;
+  float* s_l = s_m + 4 * live;
+  __syncthreads();  // scales and weights lay where the rows go
+#pragma unroll
+  for (int r = 0; r < RT; ++r) {
+    const float l = sum_xor<32>(sum_xor<16>(st.l[r]));
+    const int row = 16 * r + n;
+    if (row < live) {
+      if (g == 0) s_m[wave * live + row] = st.m[r], s_l[wave * live + row] = l;
+      float* dst = s_o + (wave * live + row) * kMaskedRowPad + 32 * g;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int c = 0; c < 8; c += 4)
+          *(mf32x4*)(dst + 8 * i + c) = mf32x4{st.o[r][c][i], st.o[r][c + 1][i], st.o[r][c + 2][i], st.o[r][c + 3][i]};
+    }
+  }
+  __syncthreads();
+  const int64_t seg = (int64_t)b * p.Hkv + h, slot = seg * p.max_pieces + piece;
+  const float vscale = SK == kScaleHead ? p.vs[h] : 1.0f;
+  for (int idx = tid; idx < live * (kHeadDim / 2); idx += 256) {
+    const int row = idx / (kHeadDim / 2), ch = 2 * (idx - row * (kHeadDim / 2));
+    float M = kNegInf, L = 0.0f, o[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int w = 0; w < 4; ++w) M = fmaxf(M, s_m[w * live + row]);
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float m = s_m[w * live + row], a = m == kNegInf ? (s_l[w * live + row] == 0.0f ? 0.0f : 1.0f) : fast_exp2(m - M);
+      const float* src = s_o + (w * live + row) * kMaskedRowPad + ch;
+      if (a != 0.0f) {
+        L = fmaf(a, s_l[w * live + row], L);
+        o[0] = fmaf(a, src[0], o[0]), o[1] = fmaf(a, src[1], o[1]);
+      }
+    }
+    const float inv = L == 0.0f ? 0.0f : vscale / L;
+    o[0] *= inv, o[1] *= inv;
+    const float lse2 = L == 0.0f ? kNegInf : (M == kNegInf ? 0.0f : M) + __log2f(L);
+    if (pieces == 1) {
+      masked_write(p, b, h, row, ch, 2, o, lse2);
+    } else {
+      ws_store2(p.ws_out + (slot * p.live_rows + row) * kHeadDim + ch, o[0], o[1]);
+      if (ch == 0) ws_store(p.ws_lse + slot * p.live_rows + row, lse2);
+    }
+  }
+  if (pieces == 1) return;
+  ws_publish();
+  __syncthreads();
+  if (tid == 0) s_last = ws_arrive(p.counters + seg) == (unsigned)pieces - 1u;
+  __syncthreads();
+  if (!s_last) return;
+  masked_combine<256>(p, b, h, 0, live, seg * p.max_pieces, pieces, tid);
+  if (tid == 0) __hip_atomic_store(p.counters + seg, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+// ---- many rows --------------------------------------------------------------------------------------------------
+
+constexpr int kMaskedItem = 8 * 64;                   // 16-byte units of one step's K or V operands in LDS
+constexpr int kMaskedChunk = 4 * kMaskedItem;         // two steps: K, K, V, V
+// Two chunks, their per-token scales, and the waves' weights of a careful pass.
+constexpr int kMaskedManyLds = 2 * kMaskedChunk * 16 + (2 * 2 * 64 + 4 * kMaskedStep * 16) * 4;
+static_assert(2 * (kMaskedManyLds + 64) <= 160 << 10, "two workgroups to a CU");
+
+// The piece's steps t0 .. t1 - 1, two at a time, folded into each wave's rows (mine: what they see).
+template <int KV, int SK, bool QS, int RT, bool CAREFUL>
+__device__ __forceinline__ void masked_many_steps(const MaskedParams& p, const MaskedRange& rg, const MaskedRange& mine, int b, int h,
+                                                  int t0, int t1, int lane, int wave, bool idle, float qs,
+                                                  const mu32x4 (&q)[RT][QS ? 8 : 4], mu32x4* s_op, float* s_scale,
+                                                  MaskedRows<RT>& st) {
+  const int my_step = wave & 1;  // this wave's share of a chunk: keys (waves 0, 1) or values (2, 3) of one step
+  masked_rows_reset(st);
+  MaskedRaw<KV> raw;
+  float sc = 0.0f;
+  auto issue = [&](int t) {  // chunk at step t of the list; steps past the piece's last repeat it
+    const int token0 = masked_token0(rg, min(t + my_step, t1 - 1));
+    const MaskedPages pages = masked_pages(p, b, token0, rg.len);
+    if (wave < 2) {
+      masked_issue_k<KV, false>(p, b, h, token0, rg.len, pages, lane, raw);
+      if constexpr (SK == kScaleTokenHead) sc = masked_issue_scale(p, b, h, token0, rg.len, pages, lane);
+    } else {
+      masked_issue_v<KV, false>(p, b, h, token0, rg.len, pages, lane, raw);
+    }
+  };
+  if (t0 < t1) issue(t0);
+  for (int t = t0, buf = 0; t < t1; t += 2, buf ^= 1) {
+    mu32x4* dst = s_op + buf * kMaskedChunk + wave * kMaskedItem + lane;
+    if (wave < 2) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int s = 0; s < 4; ++s) dst[64 * (4 * u + s)] = masked_k_frag<KV>(raw, u, s);
+      if constexpr (SK == kScaleTokenHead) s_scale[(2 * buf + wave) * 64 + lane] = sc;
+    } else {
+#pragma unroll
+      for (int c4 = 0; c4 < 2; ++c4) {
+        mu32x4 f[4];
+        masked_v_frags<KV, CAREFUL>(raw, c4, f);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) dst[64 * (4 * c4 + c)] = f[c];
+      }
+    }
+    __syncthreads();
+    if (t + 2 < t1) issue(t + 2);
+    const mu32x4* src = s_op + buf * kMaskedChunk + lane;
+#pragma unroll
+    for (int u2 = 0; u2 < 2; ++u2) {
+      const int token0 = masked_token0(rg, min(t + u2, t1 - 1));
+      if (t + u2 >= t1 || idle || masked_unseen(mine, token0)) continue;
+      mf32x4 S[RT][2];
+#pragma unroll
+      for (int r = 0; r < RT; ++r) S[r][0] = S[r][1] = mf32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+          const mu32x4 f = src[u2 * kMaskedItem + 64 * (4 * u + s)];
+#pragma unroll
+          for (int r = 0; r < RT; ++r) {
+            if constexpr (QS) S[r][u] = masked_mfma(f, q[r][4 + s], S[r][u]);
+            S[r][u] = masked_mfma(f, q[r][s], S[r][u]);
+          }
+        }
+      mu32x4 w[RT][2];
+      float* weights = s_scale + 256 + wave * kMaskedStep * 16;
+      masked_softmax<KV, SK, RT, CAREFUL>(p, mine, b, h, token0, masked_whole(mine, token0), lane, qs, s_scale + (2 * buf + u2) * 64, S, st, w,
+                                          weights);
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
+        const mu32x4 f = src[(2 + u2) * kMaskedItem + 64 * c];
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+          st.o[r][c] = masked_mfma(f, w[r][1], st.o[r][c]);
+          st.o[r][c] = masked_mfma(f, w[r][0], st.o[r][c]);
+        }
+      }
+    }
+  }
+}
+
+template <int KV, int SK, bool QS, int RT>
+__global__ __launch_bounds__(256, 2) void masked_many_kernel(const MaskedParams p) {
+  extern __shared__ mu32x4 s_op[];  // [2 chunks][K0 K1 V0 V1][8 operands][64 lanes]
+  __shared__ int s_last, s_bad;
+  constexpr int BM = 64 * RT;
+  const int tid = threadIdx.x, lane = tid & 63, wave = sread(tid >> 6);
+  const int n = lane & 15, g = lane >> 4;
+  float* s_scale = (float*)(s_op + 2 * kMaskedChunk);  // [2 chunks][2 steps][64]
+  int v = masked_index();
+  const int piece = v % p.max_pieces;
+  v /= p.max_pieces;
+  const int tile = p.tiles - 1 - v % p.tiles;  // the last rows see the most: they start first
+  v /= p.tiles;
+  const int h = v % p.Hkv, b = v / p.Hkv;
+  const int rows = p.Q * p.G, r0 = tile * BM, live = min(BM, rows - r0);
+  const MaskedRange rg = masked_range(p, b, r0, r0 + live, lane);
+  const int pieces = max((rg.n + p.piece - 1) / p.piece, 1);
+  if (piece >= pieces) return;
+  const int t0 = piece * p.piece, t1 = min(t0 + p.piece, rg.n);
+  const int first = r0 + 16 * RT * wave;  // this wave's rows
+  const bool idle = first >= rows;
+  MaskedRange mine = rg;  // what they see
+  if (!idle) masked_extent(p, b, first, min(first + 16 * RT, rows), lane, mine);
+
+  MaskedRows<RT> st;
+  masked_rows_init<RT>(p, b, h, first, rows, rg.len, lane, st);
+  mu32x4 q[RT][QS ? 8 : 4];
+  masked_load_q<KV, QS, RT>(p, b, h, first, rows, lane, q);
+  const float qs = masked_qscale<SK>(p, h);
+
+  masked_many_steps<KV, SK, QS, RT, false>(p, rg, mine, b, h, t0, t1, lane, wave, idle, qs, q, s_op, s_scale, st);
+  if (tid == 0) s_bad = 0;
+  __syncthreads();
+  if (masked_nonfinite(st)) s_bad = 1;
+  __syncthreads();
+  if (s_bad) masked_many_steps<KV, SK, QS, RT, true>(p, rg, mine, b, h, t0, t1, lane, wave, idle, qs, q, s_op, s_scale, st);
+
+  const int64_t seg = ((int64_t)b * p.Hkv + h) * p.tiles + tile, slot = seg * p.max_pieces + piece;
+  const float vscale = SK == kScaleHead ? p.vs[h] : 1.0f;
+#pragma unroll
+  for (int r = 0; r < RT; ++r) {
+    const float l = sum_xor<32>(sum_xor<16>(st.l[r]));
+    const int row = 16 * RT * wave + 16 * r + n;
+    if (row >= live) continue;
+    const float inv = l == 0.0f ? 0.0f : vscale / l;
+    const float lse2 = l == 0.0f ? kNegInf : (st.m[r] == kNegInf ? 0.0f : st.m[r]) + __log2f(l);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float o[8];
+#pragma unroll
+      for (int c = 0; c < 8; ++c) o[c] = st.o[r][c][i] * inv;
+      const int ch = 32 * g + 8 * i;
+      if (pieces == 1) {
+        masked_write(p, b, h, r0 + row, ch, 8, o, lse2);
+      } else {
+#pragma unroll
+        for (int c = 0; c < 8; c += 2) ws_store2(p.ws_out + (slot * p.live_rows + row) * kHeadDim + ch + c, o[c], o[c + 1]);
+        if (ch == 0) ws_store(p.ws_lse + slot * p.live_rows + row, lse2);
+      }
+    }
+  }
+  if (pieces == 1) return;
+  ws_publish();
+  __syncthreads();
+  if (tid == 0) s_last = ws_arrive(p.counters + seg) == (unsigned)pieces - 1u;
+  __syncthreads();
+  if (!s_last) return;
+  masked_combine<256>(p, b, h, r0, live, seg * p.max_pieces, pieces, tid);
+  if (tid == 0) __hip_atomic_store(p.counters + seg, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+// ---- launches ---------------------------------------------------------------------------------------------------
+
+template <int KV, int SK, bool QS>
+static hipError_t launch_masked_t(const MaskedParams& p, int rt, bool many, int grid, hipStream_t stream) {
+  const int live = p.live_rows;
+  // The merge's rows, or the scales and weights that lie there before it.
+  const size_t merge = (size_t)4 * live * (kMaskedRowPad + 2) * sizeof(float);
+  const size_t early = (size_t)(4 * 64 + 4 * kMaskedStep * 16) * sizeof(float);
+  const size_t few = merge > early ? merge : early;
+  const size_t lots = kMaskedManyLds;
+  const dim3 g(grid), t(256);
+  hipError_t e = hipSuccess;
+  auto allow = [&](auto kernel, size_t bytes) {  // more than 64 KiB of dynamic LDS has to be asked for, once per device
+    if (bytes > (64u << 10)) e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    return e == hipSuccess;
+  };
+  if (many && rt == 2) {
+    if (allow(masked_many_kernel<KV, SK, QS, 2>, lots)) hipLaunchKernelGGL((masked_many_kernel<KV, SK, QS, 2>), g, t, lots, stream, p);
+  } else if (many) {
+    if (allow(masked_many_kernel<KV, SK, QS, 1>, lots)) hipLaunchKernelGGL((masked_many_kernel<KV, SK, QS, 1>), g, t, lots, stream, p);
+  } else if (rt == 2) {
+    if (allow(masked_few_kernel<KV, SK, QS, 2>, few)) hipLaunchKernelGGL((masked_few_kernel<KV, SK, QS, 2>), g, t, few, stream, p);
+  } else {
+    if (allow(masked_few_kernel<KV, SK, QS, 1>, few)) hipLaunchKernelGGL((masked_few_kernel<KV, SK, QS, 1>), g, t, few, stream, p);
+  }
+  return e == hipSuccess ? hipGetLastError() : e;
+}
+
+}  // namespace bpt

@@ -1,0 +1,11 @@
+// Masked paged attention (masked_attention.h) over one cache format.
+#include "masked_attention.h"
+
+namespace bpt {
+
+hipError_t launch_masked_fp8_token(const MaskedParams& p, bool q_split, int rt, bool many, int grid, hipStream_t stream) {
+  return q_split ? launch_masked_t<kKvFp8, kScaleTokenHead, true>(p, rt, many, grid, stream)
+                 : launch_masked_t<kKvFp8, kScaleTokenHead, false>(p, rt, many, grid, stream);
+}
+
+}  // namespace bpt

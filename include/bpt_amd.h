@@ -29,6 +29,7 @@
  *                        integration/kv_cache.py:139-158 QuantizedKVCache._append quantizes completed groups.
  *   bpt_rms_norm_int8    kernels/norm_quant.py:43-109 rms_norm_int8 (kernel 1), defined by
  *                        kernels/reference.py:44-55: RMSNorm fused with per-token INT8 quantization.
+ *   bpt_paged_masked     engine/attention.py:12-47 (mask, softmax) over the paged cache, with masks and scores that it lacks.
  *   bpt_rotary_embed     engine/rope.py and the per-head norms ahead of engine/model.py:52-74's attend, one launch.
  *   bpt_rotary_append    the same, with the write half of the cache's attend (bpt_quant_append).
  */
@@ -400,6 +401,29 @@ typedef struct {
   uint8_t pair_axis[128];
 } bpt_rotary_args;
 
+/*
+ * Masks and score shaping of bpt_paged_masked, beside the bpt_decode_args of the call (whose num_splits, flags, len_offset,
+ * merge_out and merge_lse must be 0). Query i of sequence b, at position p = context_lens[b] - Q + i, sees cache slot j if
+ *   j < context_lens[b]  and  (j < prefix_lens[b]  or  (starts[b, i] <= j <= p  and  p - j < window)),
+ * and its score for head h is t = sm_scale q.k, then softcap * tanh(t / softcap), then minus slopes[h] * |p - j|. A query
+ * that sees nothing gets zeros (lse -inf).
+ *   softcap      0: none; else positive
+ *   window       0: none; else at least 1 (the query's own position counts)
+ *   slopes       float32 [Hq] or NULL
+ *   prefix_lens  int32 [B] or NULL; lengths above max_prefix are cut to it (it bounds the launch), below 0 to 0
+ *   starts       int32 [B, Q] (strides start_stride_{b,q}) or NULL
+ * q must be BF16 or F16; num_queries x num_q_heads / num_kv_heads rows are taken in tiles of 16 to 128.
+ */
+typedef struct {
+  uint32_t struct_size; /* sizeof(bpt_mask_args) */
+  float softcap;
+  int32_t window, max_prefix;
+  const float* slopes;
+  const int32_t* prefix_lens;
+  const int32_t* starts;
+  int64_t start_stride_b, start_stride_q;
+} bpt_mask_args;
+
 /* ---- entry points ------------------------------------------------------------------------------- */
 
 /* Host-only: validate args, fill chunk_tokens / grid_groups, report the workspace and counter sizes in
@@ -451,6 +475,14 @@ int bpt_kivi_quantize(const bpt_kivi_quant_args* args, void* stream);
 
 /* RMSNorm fused with per-token INT8 quantization (one launch). */
 int bpt_rms_norm_int8(const bpt_norm_quant_args* args, void* stream);
+
+/* Host-only: validate a masked call, report its workspace and counter sizes in bytes (buffers as bpt_paged_decode's). */
+int bpt_masked_plan(const bpt_decode_args* args, const bpt_mask_args* mask, size_t* workspace_bytes, size_t* counters_bytes);
+
+/* Paged attention with a score cap, a bias that falls with distance, a window, a prefix that every query sees and a first
+ * token per query: one launch, any number of queries. No counterpart among the reference's kernels, whose attention knows
+ * the causal mask (engine/attention.py:12-47). */
+int bpt_paged_masked(const bpt_decode_args* args, const bpt_mask_args* mask, void* stream);
 
 /* Queries and keys normalised and rotated by their positions: one launch. No counterpart among the reference's kernels; its
  * model does this in torch ahead of the cache's attend (engine/model.py:52-74, engine/rope.py). */

@@ -374,10 +374,12 @@ struct MaskedParams {
   float* ws_out;       // [segments, max_pieces, live_rows, D] normalized partials
   float* ws_lse;       // [segments, max_pieces, live_rows] their log2-sum-exp
   unsigned* counters;  // [segments] arrivals; zero between calls
-  int Q, Hq, Hkv, G, P, logP, num_blocks, len_cap, table_i64, out_dtype;
+  int B, Q, Hq, Hkv, G, P, logP, num_blocks, len_cap, table_i64, out_dtype;
   int window;      // 0: none
   int max_prefix;  // prefix lengths above it are cut to it
   int tiles;       // row tiles of a KV head
+  unsigned G_inv;  // ceil(2^32 / G): r / G is the high word of its product with r
+  int out_pairs;   // out's rows lie on 4-byte boundaries (16-bit outputs)
   int live_rows;   // rows of the largest tile
   int piece;       // steps of a piece
   int max_pieces;  // pieces of the longest tile

@@ -1016,6 +1016,7 @@ int masked_setup(const bpt_decode_args* a, const bpt_mask_args* m, const char* f
     return fail(BPT_ERR_INVALID_ARGUMENT, "%s: 16 tokens of a page must lie within 2 GiB", fn);
 
   bpt::MaskedParams p{};
+  p.B = a->batch;
   p.Q = a->num_queries;
   p.Hq = a->num_q_heads;
   p.Hkv = a->num_kv_heads;
@@ -1039,6 +1040,9 @@ int masked_setup(const bpt_decode_args* a, const bpt_mask_args* m, const char* f
   plan->many = rows > 32;
   plan->rt = plan->many ? (rows > 64 ? 2 : 1) : (rows > 16 ? 2 : 1);
   const int tile = plan->many ? 64 * plan->rt : rows;
+  if ((int64_t)rows * p.G > 0x7fffffffLL)  // row / G is exact below that
+    return fail(BPT_ERR_INVALID_ARGUMENT, "%s: too many rows", fn);
+  p.G_inv = (unsigned)((((uint64_t)1 << 32) + p.G - 1) / p.G);
   p.tiles = (rows + tile - 1) / tile;
   p.live_rows = std::min(rows, tile);
   // Steps of a tile at most: the prefix's, and those from the first token that the window leaves its first query to its last
@@ -1056,8 +1060,8 @@ int masked_setup(const bpt_decode_args* a, const bpt_mask_args* m, const char* f
   p.piece = (int)std::min<int64_t>(piece, 1 << 26);
   p.max_pieces = (int)std::max<int64_t>(1, (steps + p.piece - 1) / p.piece);
   const int64_t slots = segments * p.max_pieces;
-  if (slots > 0x7fffffffLL) return fail(BPT_ERR_INVALID_ARGUMENT, "%s: batch x heads x rows too large", fn);
-  plan->grid = (int)slots;
+  if (slots > 0x70000000LL) return fail(BPT_ERR_INVALID_ARGUMENT, "%s: batch x heads x rows too large", fn);
+  plan->grid = (int)(plan->many ? slots : ((int64_t)a->batch * p.max_pieces + 7) / 8 * 8 * p.Hkv);  // few rows: see the kernel
   plan->ws_out_floats = p.max_pieces > 1 ? (size_t)slots * p.live_rows * a->head_dim : 0;
   plan->workspace = p.max_pieces > 1 ? align256((plan->ws_out_floats + (size_t)slots * p.live_rows) * sizeof(float)) : 0;
   plan->counters = p.max_pieces > 1 ? align256((size_t)segments * sizeof(unsigned)) : 0;
@@ -1122,6 +1126,7 @@ int bpt_paged_masked(const bpt_decode_args* a, const bpt_mask_args* m, void* str
   p.o_sq = a->out_stride_q;
   p.o_sh = a->out_stride_h;
   p.out_dtype = a->out_dtype;
+  p.out_pairs = ((uintptr_t)a->out & 3u) == 0 && a->out_stride_b % 2 == 0 && a->out_stride_q % 2 == 0 && a->out_stride_h % 2 == 0;
   p.lse_out = a->lse_out;
   p.slopes = m->slopes;
   p.prefix_lens = m->prefix_lens;

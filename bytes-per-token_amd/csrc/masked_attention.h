@@ -33,6 +33,8 @@
 // Finite data pays one look at the result.
 #pragma once
 
+#include <type_traits>
+
 #include "decode_common.h"
 
 namespace bpt {
@@ -43,6 +45,8 @@ typedef uint32_t mu32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t mu32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kMaskedStep = 32;
+constexpr int kMaskedRowPad = kHeadDim + 4;  // floats of a row in LDS: 16 rows spread over the banks
+constexpr int kMaskedItem = 8 * 64;  // 16-byte units of one step's K or V operands in LDS
 constexpr float kMaskedSlack = 8.0f;  // a row's reference point may lag its maximum by this (log2): weights stay below 2^8
 
 // ---- conversions ------------------------------------------------------------------------------------------------
@@ -97,22 +101,12 @@ struct MaskedRaw {
   uint32_t w[kWords];
 };
 
-// The pages (clamped into the pool) of a step's two 16-token groups, for page sizes of at least 16.
+// The pages of a step's two 16-token groups, for page sizes of at least 16.
 struct MaskedPages {
   int e[2];
 };
 __device__ __forceinline__ int masked_clamp_page(const MaskedParams& p, int e) {
   return e < 0 ? 0 : (e >= p.num_blocks ? p.num_blocks - 1 : e);
-}
-__device__ __forceinline__ MaskedPages masked_pages(const MaskedParams& p, int b, int token0, int len) {
-  MaskedPages g{{0, 0}};
-  if (p.logP >= 4) {
-    const int32_t* table = (const int32_t*)p.table;
-#pragma unroll
-    for (int t = 0; t < 2; ++t)
-      g.e[t] = load_uniform(table + (((int64_t)b * p.table_sb + (min(token0 + 16 * t, len - 1) >> p.logP)) << p.table_i64));
-  }
-  return g;
 }
 // Byte offset of a token's row of head h in the pools (any page size). Tokens past the last one read it instead.
 __device__ __forceinline__ int64_t masked_row(const MaskedParams& p, int b, int h, int token, int len) {
@@ -136,29 +130,27 @@ __device__ __forceinline__ void masked_load(const uint8_t* src, uint32_t* w) {
   for (int i = 0; i < W; ++i) w[i] = x[i];
 }
 
-// Keys: lane (n, g) takes token n of both 16-token groups; of bf16 channels 32 s + 8 g .. + 7 for product s, of codes
-// 64 j + 16 g .. + 15 for products 2 j and 2 j + 1.
-template <int KV, bool ONCE>
+// Keys: whole rows, 16 bytes a lane (of codes, 8 lanes to a token and 8 tokens to a load; of bf16, 16 and 4), which the memory
+// pipeline serves faster than the operands' own order. They get into that order through LDS (masked_k_place).
+template <int KV, bool PU, bool ONCE>
 __device__ __forceinline__ void masked_issue_k(const MaskedParams& p, int b, int h, int token0, int len, MaskedPages pages,
                                                int lane, MaskedRaw<KV>& r) {
-  constexpr int KL = KV == kKvBf16 ? 4 : 2;
-  const int n = lane & 15, g = lane >> 4;
+  constexpr int S = KV == kKvBf16 ? 16 : 8, PER = 64 / S;  // 16-byte segments of a row, rows of a load
+  const int row = lane / S, seg = lane % S;
 #pragma unroll
   for (int t = 0; t < 2; ++t) {
-    const uint8_t* src;
-    if (p.logP >= 4) {
-      int rmax;
-      const int64_t base = masked_group(p, h, pages.e[t], token0 + 16 * t, len, rmax);
-      src = p.k + base + (uint32_t)(min(n, rmax) * (uint32_t)p.kv_stok + 16 * g);
-    } else {
-      src = p.k + masked_row(p, b, h, token0 + 16 * t + n, len) + 16 * g;
-    }
+    int rmax = 0;
+    const int64_t base = PU ? masked_group(p, h, pages.e[t], token0 + 16 * t, len, rmax) : 0;
 #pragma unroll
-    for (int j = 0; j < KL; ++j) masked_load<4, ONCE>(src + 64 * j, r.w + 4 * (KL * t + j));
+    for (int j = 0; j < 16 / PER; ++j) {
+      const uint8_t* src = PU ? p.k + base + (uint32_t)(min(PER * j + row, rmax) * (uint32_t)p.kv_stok + 16 * seg)
+                                       : p.k + masked_row(p, b, h, token0 + 16 * t + PER * j + row, len) + 16 * seg;
+      masked_load<4, ONCE>(src, r.w + 4 * (16 / PER * t + j));
+    }
   }
 }
 // Values: lane (n, g) takes channels 8 n .. + 7 of tokens 4 g + i and 16 + 4 g + i.
-template <int KV, bool ONCE>
+template <int KV, bool PU, bool ONCE>
 __device__ __forceinline__ void masked_issue_v(const MaskedParams& p, int b, int h, int token0, int len, MaskedPages pages,
                                                int lane, MaskedRaw<KV>& r) {
   constexpr int W = KV == kKvBf16 ? 4 : 2;
@@ -166,36 +158,55 @@ __device__ __forceinline__ void masked_issue_v(const MaskedParams& p, int b, int
 #pragma unroll
   for (int t = 0; t < 2; ++t) {
     int rmax = 0;
-    const int64_t base = p.logP >= 4 ? masked_group(p, h, pages.e[t], token0 + 16 * t, len, rmax) : 0;
+    const int64_t base = PU ? masked_group(p, h, pages.e[t], token0 + 16 * t, len, rmax) : 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const uint8_t* src = p.logP >= 4 ? p.v + base + (uint32_t)(min(4 * g + i, rmax) * (uint32_t)p.kv_stok + 4 * W * n)
+      const uint8_t* src = PU ? p.v + base + (uint32_t)(min(4 * g + i, rmax) * (uint32_t)p.kv_stok + 4 * W * n)
                                        : p.v + masked_row(p, b, h, token0 + 16 * t + 4 * g + i, len) + 4 * W * n;
       masked_load<W, ONCE>(src, r.w + W * (4 * t + i));
     }
   }
 }
 // Per-token scales: lane l < 32 takes the key's scale of token l, the others the value's of token l - 32.
+template <bool PU>
 __device__ __forceinline__ float masked_issue_scale(const MaskedParams& p, int b, int h, int token0, int len, MaskedPages pages,
                                                     int lane) {
   const int tok = min(token0 + (lane & 31), len - 1);
   int e;
-  if (p.logP >= 4) e = (lane & 16) ? pages.e[1] : pages.e[0];
+  if (PU) e = (lane & 16) ? pages.e[1] : pages.e[0];
   else e = ((const int32_t*)p.table)[((int64_t)b * p.table_sb + (tok >> p.logP)) << p.table_i64];
   return (lane < 32 ? p.ks : p.vs)[(int64_t)masked_clamp_page(p, e) * p.sc_sblk + (int64_t)(tok & (p.P - 1)) * p.sc_stok +
                                    (int64_t)h * p.sc_shead];
 }
 
-// The key operand of product s over 16-token group t.
+// Loaded key rows into LDS as the first product's operands: operand s of 16-token group t is 64 units of 16 bytes, unit 16 g + n
+// for lane (n, g), from `dst` + 64 (4 t + s) on. Product s takes channels 32 s + 8 g .. + 7 of bf16 rows (segment 4 s + g), of codes
+// 64 (s / 2) + 16 g + 8 (s % 2) .. + 7 (halves of segment 4 (s / 2) + g). Units are permuted within their eights by segment, so
+// that the 8 lanes that store a row's segments, and the 8 that read one of 8 rows, touch all banks.
+__device__ __forceinline__ int masked_k_unit(int t, int s, int g, int n, int twist) {
+  return 64 * (4 * t + s) + ((16 * g + n) ^ (g + 4 * twist));
+}
 template <int KV>
-__device__ __forceinline__ mu32x4 masked_k_frag(const MaskedRaw<KV>& r, int t, int s) {
-  if constexpr (KV == kKvBf16) {
-    const uint32_t* w = r.w + 4 * (4 * t + s);
-    return mu32x4{w[0], w[1], w[2], w[3]};
-  } else {
-    const uint32_t* w = r.w + 4 * (2 * t + (s >> 1)) + 2 * (s & 1);
-    return masked_codes8<KV>(w[0], w[1]);
-  }
+__device__ __forceinline__ void masked_k_place(const MaskedRaw<KV>& r, int lane, mu32x4* dst) {
+  constexpr int S = KV == kKvBf16 ? 16 : 8, PER = 64 / S;
+  const int row = lane / S, seg = lane % S;
+#pragma unroll
+  for (int t = 0; t < 2; ++t)
+#pragma unroll
+    for (int j = 0; j < 16 / PER; ++j) {
+      const uint32_t* w = r.w + 4 * (16 / PER * t + j);
+      const int n = PER * j + row, g = seg & 3, s = seg >> 2;
+      if constexpr (KV == kKvBf16) {
+        dst[masked_k_unit(t, s, g, n, s & 1)] = mu32x4{w[0], w[1], w[2], w[3]};
+      } else {
+        dst[masked_k_unit(t, 2 * s, g, n, s)] = masked_codes8<KV>(w[0], w[1]);
+        dst[masked_k_unit(t, 2 * s + 1, g, n, s)] = masked_codes8<KV>(w[2], w[3]);
+      }
+    }
+}
+template <int KV>
+__device__ __forceinline__ mu32x4 masked_k_frag(const mu32x4* src, int t, int s, int lane) {
+  return src[masked_k_unit(t, s, lane >> 4, lane & 15, KV == kKvBf16 ? s & 1 : s >> 1)];
 }
 // The value operands of four channel blocks c = 4 q .. 4 q + 3: channel 8 n + c of the lane's 8 tokens. CAREFUL: with values
 // that are not finite replaced by zeros.
@@ -244,6 +255,18 @@ struct MaskedRange {
   int min_lo, max_hi;   // some row sees tokens min_lo .. max_hi - 1 behind the prefix
 };
 __device__ __forceinline__ int masked_token0(const MaskedRange& r, int t) { return kMaskedStep * (t < r.sa ? t : r.sb + t - r.sa); }
+
+// The page ids of step t's two 16-token groups, in lanes 0 and 1, and of step t + stride's, in lanes 2 and 3 (both clamped to the
+// piece's last step), on their way for masked_pages. (Scalar loads would share their counter with LDS: every read of that would wait for the page table.)
+template <bool PU>
+__device__ __forceinline__ int masked_page_list(const MaskedParams& p, const MaskedRange& r, int b, int t, int stride, int t1, int lane) {
+  if (!PU) return 0;
+  const int token = masked_token0(r, min(t + (lane & 2 ? stride : 0), t1 - 1)) + 16 * (lane & 1);
+  return ((const int32_t*)p.table)[((int64_t)b * p.table_sb + (min(token, r.len - 1) >> p.logP)) << p.table_i64];
+}
+__device__ __forceinline__ MaskedPages masked_pages(int list, int which = 0) {
+  return MaskedPages{{__builtin_amdgcn_readlane(list, 2 * which), __builtin_amdgcn_readlane(list, 2 * which + 1)}};
+}
 
 __device__ __forceinline__ void masked_bounds(const MaskedParams& p, int b, int qi, int len, int& pos, int& lo, int& hi) {
   pos = len - p.Q + qi;
@@ -298,13 +321,16 @@ __device__ __forceinline__ bool masked_unseen(const MaskedRange& r, int token0) 
   return token0 >= r.prefix && (token0 >= r.max_hi || token0 + kMaskedStep <= r.min_lo);
 }
 
+// Row r's query, r / G by a multiplication (the host checks that it is exact).
+__device__ __forceinline__ int masked_query(const MaskedParams& p, int r) { return p.G == 1 ? r : (int)__umulhi((unsigned)r, p.G_inv); }
+
 template <int RT>
 __device__ __forceinline__ void masked_rows_init(const MaskedParams& p, int b, int h, int first, int rows, int len, int lane,
                                                  MaskedRows<RT>& s) {
 #pragma unroll
   for (int t = 0; t < RT; ++t) {
     const int r = min(first + 16 * t + (lane & 15), rows - 1);  // lanes past the last row repeat it
-    const int qi = r / p.G;
+    const int qi = masked_query(p, r);
     masked_bounds(p, b, qi, len, s.pos[t], s.lo[t], s.hi[t]);
     s.slope[t] = p.slopes ? p.slopes[h * p.G + r - qi * p.G] * kLog2e : 0.0f;
   }
@@ -327,7 +353,7 @@ __device__ __forceinline__ void masked_load_q(const MaskedParams& p, int b, int 
 #pragma unroll
   for (int t = 0; t < RT; ++t) {
     const int r = min(first + 16 * t + (lane & 15), rows - 1);
-    const int qi = r / p.G;
+    const int qi = masked_query(p, r);
     const uint16_t* src = (const uint16_t*)p.q + (int64_t)b * p.q_sb + (int64_t)qi * p.q_sq + (int64_t)(h * p.G + r - qi * p.G) * p.q_sh;
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
@@ -385,6 +411,11 @@ __device__ __forceinline__ void masked_add_nonfinite(const MaskedParams& p, int 
   }
 }
 
+// cap tanh(t / cap) from u = 2 log2e t / cap.
+__device__ __forceinline__ float masked_cap(float cap, float u) {
+  return fmaf(-2.0f * cap, __builtin_amdgcn_rcpf(1.0f + fast_exp2(u)), cap);
+}
+
 // Scores S[rt][t] (token 16 t + 4 g + i, raw products) -> weights' two bf16 parts w[rt][part], the rows' state brought up to
 // date. sc: per-token scales of the step (keys' 32, then values' 32). careful (uniform): values that are not finite stay out of
 // the products and are added here instead (weights: this wave's 512 floats of LDS for that).
@@ -408,18 +439,17 @@ __device__ __forceinline__ void masked_softmax(const MaskedParams& p, const Mask
     float x[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) x[e] = S[r][e >> 2][e & 3] * (SK == kScaleTokenHead ? kf[e] : qs);
-    if (p.cap > 0.0f) {
+    if (p.cap > kMaskedPlainCap) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float u = x[e];  // 2 log2e t / cap
-        const float y = p.cap - 2.0f * p.cap * __builtin_amdgcn_rcpf(1.0f + fast_exp2(u));
-        x[e] = y;
-        if (p.cap > kMaskedPlainCap) {  // tanh z = z (1 - z^2 / 3 + 2 z^4 / 15 - 17 z^6 / 315), z = u ln2 / 2
-          const float z = u * (0.5f * kLn2), z2 = z * z;
-          const float series = fmaf(z2, fmaf(z2, fmaf(z2, -17.0f / 315.0f, 2.0f / 15.0f), -1.0f / 3.0f), 1.0f);
-          if (fabsf(z) < 0.25f) x[e] = p.cap * z * series;
-        }
+      for (int e = 0; e < 8; ++e) {  // tanh z = z (1 - z^2 / 3 + 2 z^4 / 15 - 17 z^6 / 315) near 0, z = u ln2 / 2
+        const float z = x[e] * (0.5f * kLn2), z2 = z * z;
+        const float series = fmaf(z2, fmaf(z2, fmaf(z2, -17.0f / 315.0f, 2.0f / 15.0f), -1.0f / 3.0f), 1.0f);
+        const float y = masked_cap(p.cap, x[e]);
+        x[e] = fabsf(z) < 0.25f ? p.cap * z * series : y;
       }
+    } else if (p.cap > 0.0f) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = masked_cap(p.cap, x[e]);
     }
     if (p.slopes) {
       const float d0 = (float)(st.pos[r] - token0 - 4 * g);
@@ -502,51 +532,81 @@ __device__ __forceinline__ float masked_qscale(const MaskedParams& p, int h) {
   return SK == kScaleHead ? p.qscale * p.ks[h] : p.qscale;
 }
 
-// One output element's row, and a lane's 32 channels of it from `ch` on.
-__device__ __forceinline__ void masked_write(const MaskedParams& p, int b, int h, int r, int ch, int count, const float* o, float lse2) {
-  const int qi = r / p.G, hq = h * p.G + r - qi * p.G;
-  const int64_t at = (int64_t)b * p.o_sb + (int64_t)qi * p.o_sq + (int64_t)hq * p.o_sh + ch;
-  for (int i = 0; i < count; ++i) store_float(p.out, at + i, p.out_dtype, o[i]);
-  if (p.lse_out && ch == 0) p.lse_out[((int64_t)b * p.Q + qi) * p.Hq + hq] = lse2 == kNegInf ? kNegInf : lse2 * kLn2;
+// Sixteen lanes to a row from here on: lane c of them takes channel pairs 2 c + 32 i, so that every store and load of theirs is
+// one piece of memory.
+struct MaskedPairs {
+  float x[4][2];
+};
+__device__ __forceinline__ void masked_store_pairs(const MaskedParams& p, int b, int h, int r, int c, const MaskedPairs& o, float lse2) {
+  const int qi = masked_query(p, r), hq = h * p.G + r - qi * p.G;
+  const int64_t at = (int64_t)b * p.o_sb + (int64_t)qi * p.o_sq + (int64_t)hq * p.o_sh + 2 * c;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (!p.out_pairs || p.out_dtype == kFF32) {
+      store_float(p.out, at + 32 * i, p.out_dtype, o.x[i][0]);
+      store_float(p.out, at + 32 * i + 1, p.out_dtype, o.x[i][1]);
+    } else {
+      const uint32_t w = p.out_dtype == kFBf16 ? __builtin_bit_cast(uint32_t, pack_bf16(o.x[i][0], o.x[i][1]))
+                                               : __builtin_bit_cast(uint32_t, f16x2{(_Float16)o.x[i][0], (_Float16)o.x[i][1]});
+      *(uint32_t*)((uint16_t*)p.out + at + 32 * i) = w;
+    }
+  }
+  if (p.lse_out && c == 0) p.lse_out[((int64_t)b * p.Q + qi) * p.Hq + hq] = lse2 == kNegInf ? kNegInf : lse2 * kLn2;
+}
+__device__ __forceinline__ void masked_store_partial(const MaskedParams& p, int64_t slot, int row, int c, const MaskedPairs& o, float lse2) {
+  float* dst = p.ws_out + (slot * p.live_rows + row) * kHeadDim + 2 * c;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) ws_store2(dst + 32 * i, o.x[i][0], o.x[i][1]);
+  if (c == 0) ws_store(p.ws_lse + slot * p.live_rows + row, lse2);
 }
 
-// A tile's n pieces (slots slot0 ..) combined by the last of them to arrive, the whole workgroup of NT threads: two channels of
-// a row a thread, the pieces in order, so that the sum does not depend on who came last.
+// A tile's n pieces (slots slot0 ..) combined by the last of them to arrive, in order, so that the sum does not depend on who came
+// last: the whole workgroup of NT threads. Four pieces' loads are under way together: a round trip to the memory side takes
+// microseconds.
 template <int NT>
 __device__ __forceinline__ void masked_combine(const MaskedParams& p, int b, int h, int r0, int live, int64_t slot0, int n, int tid) {
   ws_acquire();
-  for (int idx = tid; idx < live * (kHeadDim / 2); idx += NT) {
-    const int row = idx / (kHeadDim / 2), ch = 2 * (idx - row * (kHeadDim / 2));
+  constexpr int NP = 4;
+  const int c = tid & 15;
+  for (int row = tid >> 4; row < live; row += NT / 16) {
     const float* lse = p.ws_lse + slot0 * p.live_rows + row;
-    const float* prt = p.ws_out + (slot0 * p.live_rows + row) * kHeadDim + ch;
-    float M = kNegInf, W = 0.0f, o[2] = {0.0f, 0.0f};
-    for (int j0 = 0; j0 < n; j0 += 8) {
-      float lv[8], ov[8][2], top = kNegInf;
+    const float* prt = p.ws_out + (slot0 * p.live_rows + row) * kHeadDim + 2 * c;
+    float M = kNegInf, W = 0.0f;
+    MaskedPairs o{};
+    for (int j0 = 0; j0 < n; j0 += NP) {
+      float lv[NP], top = kNegInf;
+      MaskedPairs ov[NP];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        lv[j] = kNegInf, ov[j][0] = ov[j][1] = 0.0f;
+      for (int j = 0; j < NP; ++j) {
+        lv[j] = kNegInf;
         if (j0 + j < n) {
           lv[j] = ws_load(lse + (int64_t)(j0 + j) * p.live_rows);
-          ws_load2(prt + (int64_t)(j0 + j) * p.live_rows * kHeadDim, ov[j][0], ov[j][1]);
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            ws_load2(prt + (int64_t)(j0 + j) * p.live_rows * kHeadDim + 32 * i, ov[j].x[i][0], ov[j].x[i][1]);
         }
       }
 #pragma unroll
-      for (int j = 0; j < 8; ++j) top = fmaxf(top, lv[j]);
+      for (int j = 0; j < NP; ++j) top = fmaxf(top, lv[j]);
       const float nm = fmaxf(M, top), mu = nm == kNegInf ? 0.0f : nm;
       const float a = W > 0.0f ? fast_exp2(M - mu) : (W != W ? W : 0.0f);
-      W *= a, o[0] *= a, o[1] *= a;
+      W *= a;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
+      for (int i = 0; i < 4; ++i) o.x[i][0] *= a, o.x[i][1] *= a;
+#pragma unroll
+      for (int j = 0; j < NP; ++j) {
         if (lv[j] == kNegInf) continue;  // an empty piece
         const float e = fast_exp2(lv[j] - mu);
         W += e;
-        o[0] = fmaf(e, ov[j][0], o[0]), o[1] = fmaf(e, ov[j][1], o[1]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o.x[i][0] = fmaf(e, ov[j].x[i][0], o.x[i][0]), o.x[i][1] = fmaf(e, ov[j].x[i][1], o.x[i][1]);
       }
       M = nm;
     }
-    const float inv = W == 0.0f ? 0.0f : 1.0f / W;
-    o[0] *= inv, o[1] *= inv;
-    masked_write(p, b, h, r0 + row, ch, 2, o, W == 0.0f ? kNegInf : M + __log2f(W));
+    const float inv = W == 0.0f ? 0.0f : __builtin_amdgcn_rcpf(W);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o.x[i][0] *= inv, o.x[i][1] *= inv;
+    masked_store_pairs(p, b, h, r0 + row, c, o, W == 0.0f ? kNegInf : M + __log2f(W));
   }
 }
 
@@ -560,25 +620,36 @@ __device__ __forceinline__ int masked_index() {
 
 // ---- few rows ---------------------------------------------------------------------------------------------------
 
-constexpr int kMaskedRowPad = kHeadDim + 4;  // floats of a row in LDS: 16 rows spread over the banks
-
-// One wave's steps t0 + wave, t0 + wave + 4, ... < t1 folded into its rows. The next step's codes are requested as soon as the
-// registers of this one's are free.
-template <int KV, int SK, bool QS, int RT, bool CAREFUL>
+// One wave's steps t, t + 4, ... < t1 folded into its rows. The next step's keys are requested once this one's have gone to LDS,
+// its values once this one's are multiplied, and the page ids of the step after that in between: no request stands behind a
+// branch, so that each is waited for by itself.
+template <int KV, int SK, bool PU, bool QS, int RT, bool CAREFUL>
 __device__ __forceinline__ void masked_few_steps(const MaskedParams& p, const MaskedRange& rg, int b, int h, int t, int t1, int lane,
-                                                 float qs, const mu32x4 (&q)[RT][QS ? 8 : 4], float* w_scale, float* w_weights,
-                                                 MaskedRows<RT>& st) {
+                                                 float qs, const mu32x4 (&q)[RT][QS ? 8 : 4], mu32x4* w_keys, float* w_scale,
+                                                 float* w_weights, MaskedRows<RT>& st) {
   masked_rows_reset(st);
   if (t >= t1) return;
-  MaskedRaw<KV> k, vv;
+  MaskedRaw<KV> k, v;
   float sc = 0.0f;
   int token0 = masked_token0(rg, t);
-  MaskedPages pages = masked_pages(p, b, token0, rg.len);
-  masked_issue_k<KV, true>(p, b, h, token0, rg.len, pages, lane, k);
-  masked_issue_v<KV, true>(p, b, h, token0, rg.len, pages, lane, vv);
-  if constexpr (SK == kScaleTokenHead) sc = masked_issue_scale(p, b, h, token0, rg.len, pages, lane);
-  pages = masked_pages(p, b, masked_token0(rg, min(t + 4, t1 - 1)), rg.len);
-  for (; t < t1; t += 4) {
+  int list = masked_page_list<PU>(p, rg, b, t, 4, t1, lane);
+  MaskedPages pages = masked_pages(list, 1);  // the next step's
+  {
+    const MaskedPages pages = masked_pages(list);
+    masked_issue_k<KV, PU, true>(p, b, h, token0, rg.len, pages, lane, k);
+    if constexpr (SK == kScaleTokenHead) sc = masked_issue_scale<PU>(p, b, h, token0, rg.len, pages, lane);
+    masked_issue_v<KV, PU, true>(p, b, h, token0, rg.len, pages, lane, v);
+  }
+  auto step = [&](auto last) {
+    masked_k_place<KV>(k, lane, w_keys);
+    if constexpr (SK == kScaleTokenHead) w_scale[lane] = sc;
+    const int next = last ? 0 : masked_token0(rg, t + 4);
+    if constexpr (!last) {
+      masked_issue_k<KV, PU, true>(p, b, h, next, rg.len, pages, lane, k);
+      if constexpr (SK == kScaleTokenHead) sc = masked_issue_scale<PU>(p, b, h, next, rg.len, pages, lane);
+      list = masked_page_list<PU>(p, rg, b, t + 8, 0, t1, lane);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // the wave's lanes read one another's
     mf32x4 S[RT][2];
 #pragma unroll
     for (int r = 0; r < RT; ++r) S[r][0] = S[r][1] = mf32x4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -586,26 +657,19 @@ __device__ __forceinline__ void masked_few_steps(const MaskedParams& p, const Ma
     for (int u = 0; u < 2; ++u)
 #pragma unroll
       for (int s = 0; s < 4; ++s) {
-        const mu32x4 f = masked_k_frag<KV>(k, u, s);
+        const mu32x4 f = masked_k_frag<KV>(w_keys, u, s, lane);
 #pragma unroll
         for (int r = 0; r < RT; ++r) {
           if constexpr (QS) S[r][u] = masked_mfma(f, q[r][4 + s], S[r][u]);
           S[r][u] = masked_mfma(f, q[r][s], S[r][u]);
         }
       }
-    const int next = masked_token0(rg, min(t + 4, t1 - 1));
-    if (t + 4 < t1) masked_issue_k<KV, true>(p, b, h, next, rg.len, pages, lane, k);
-    if constexpr (SK == kScaleTokenHead) {
-      w_scale[lane] = sc;
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      if (t + 4 < t1) sc = masked_issue_scale(p, b, h, next, rg.len, pages, lane);
-    }
     mu32x4 w[RT][2];
     masked_softmax<KV, SK, RT, CAREFUL>(p, rg, b, h, token0, masked_whole(rg, token0), lane, qs, w_scale, S, st, w, w_weights);
 #pragma unroll
     for (int c4 = 0; c4 < 2; ++c4) {
       mu32x4 f[4];
-      masked_v_frags<KV, CAREFUL>(vv, c4, f);
+      masked_v_frags<KV, CAREFUL>(v, c4, f);
 #pragma unroll
       for (int c = 0; c < 4; ++c)
 #pragma unroll
@@ -614,22 +678,30 @@ __device__ __forceinline__ void masked_few_steps(const MaskedParams& p, const Ma
           st.o[r][4 * c4 + c] = masked_mfma(f[c], w[r][0], st.o[r][4 * c4 + c]);
         }
     }
-    if (t + 4 < t1) masked_issue_v<KV, true>(p, b, h, next, rg.len, pages, lane, vv);
-    pages = masked_pages(p, b, masked_token0(rg, min(t + 8, t1 - 1)), rg.len);
-    token0 = next;
-  }
+    if constexpr (!last) {
+      masked_issue_v<KV, PU, true>(p, b, h, next, rg.len, pages, lane, v);
+      pages = masked_pages(list);
+      token0 = next;
+    }
+  };
+  for (; t + 4 < t1; t += 4) step(std::false_type{});
+  step(std::true_type{});
 }
 
-template <int KV, int SK, bool QS, int RT>
+template <int KV, int SK, bool PU, bool QS, int RT>
 __global__ __launch_bounds__(256, RT == 1 ? 3 : 2) void masked_few_kernel(const MaskedParams p) {
-  extern __shared__ float smem[];  // [4 waves][live][kMaskedRowPad], then [4 waves][live] m and l; scales and weights on the way
+  // [4 waves][live][kMaskedRowPad], then [live][4] m and l; on the way there key operands, scales and weights. Vectors, so that it
+  // lies on a 16-byte boundary whatever other LDS there is: 16-byte accesses off it take eight times as long.
+  extern __shared__ mf32x4 s_dyn[];
+  float* smem = (float*)s_dyn;
   __shared__ int s_last;
   const int tid = threadIdx.x, lane = tid & 63, wave = sread(tid >> 6);
   const int n = lane & 15, g = lane >> 4;
-  int v = masked_index();
-  const int h = v % p.Hkv;
-  v /= p.Hkv;
-  const int piece = v % p.max_pieces, b = v / p.max_pieces;
+  // Workgroups go to the 8 XCDs in turn: the heads of a piece, whose rows share pages and lines of scales, go to one, and the
+  // pieces are dealt out to the XCDs in turn, the first ones of all sequences before the second ones.
+  const int turn = (blockIdx.x >> 3) / p.Hkv * 8 + (blockIdx.x & 7), h = (blockIdx.x >> 3) % p.Hkv;
+  const int piece = turn / p.B, b = turn % p.B;
+  if (piece >= p.max_pieces) return;
   const int rows = p.Q * p.G;
   const MaskedRange rg = masked_range(p, b, 0, rows, lane);
   const int pieces = max((rg.n + p.piece - 1) / p.piece, 1);
@@ -642,24 +714,25 @@ __global__ __launch_bounds__(256, RT == 1 ? 3 : 2) void masked_few_kernel(const 
   mu32x4 q[RT][QS ? 8 : 4];
   masked_load_q<KV, QS, RT>(p, b, h, 0, rows, lane, q);
   const float qs = masked_qscale<SK>(p, h);
-  float* w_scale = smem + wave * 64;                             // this wave's per-token scales
-  float* w_weights = smem + 4 * 64 + wave * kMaskedStep * 16;  // and, where needed, its weights
+  mu32x4* w_keys = (mu32x4*)smem + wave * kMaskedItem;  // this wave's key operands,
+  float* w_scale = smem + 4 * 4 * kMaskedItem + wave * 64;  // per-token scales
+  float* w_weights = smem + 4 * 4 * kMaskedItem + 4 * 64 + wave * kMaskedStep * 16;  // and, where needed, weights
 
-  masked_few_steps<KV, SK, QS, RT, false>(p, rg, b, h, t0 + wave, t1, lane, qs, q, w_scale, w_weights, st);
+  masked_few_steps<KV, SK, PU, QS, RT, false>(p, rg, b, h, t0 + wave, t1, lane, qs, q, w_keys, w_scale, w_weights, st);
   if (__any(masked_nonfinite(st)))
-    masked_few_steps<KV, SK, QS, RT, true>(p, rg, b, h, t0 + wave, t1, lane, qs, q, w_scale, w_weights, st);
+    masked_few_steps<KV, SK, PU, QS, RT, true>(p, rg, b, h, t0 + wave, t1, lane, qs, q, w_keys, w_scale, w_weights, st);
 
   // The waves' shares of each row, brought to the row's maximum and added.
-  float* s_o = smem;
-  float* s_m = smem + 4 * live * kMaskedRowPad;
+  float* s_o = smem;                             // [4 waves][live][kMaskedRowPad]
+  float* s_m = smem + 4 * live * kMaskedRowPad;  // [live][4 waves]
   float* s_l = s_m + 4 * live;
-  __syncthreads();  // scales and weights lay where the rows go
+  __syncthreads();  // keys, scales and weights lay where the rows go
 #pragma unroll
   for (int r = 0; r < RT; ++r) {
     const float l = sum_xor<32>(sum_xor<16>(st.l[r]));
     const int row = 16 * r + n;
     if (row < live) {
-      if (g == 0) s_m[wave * live + row] = st.m[r], s_l[wave * live + row] = l;
+      if (g == 0) s_m[4 * row + wave] = st.m[r], s_l[4 * row + wave] = l;
       float* dst = s_o + (wave * live + row) * kMaskedRowPad + 32 * g;
 #pragma unroll
       for (int i = 0; i < 4; ++i)
@@ -671,29 +744,32 @@ __global__ __launch_bounds__(256, RT == 1 ? 3 : 2) void masked_few_kernel(const 
   __syncthreads();
   const int64_t seg = (int64_t)b * p.Hkv + h, slot = seg * p.max_pieces + piece;
   const float vscale = SK == kScaleHead ? p.vs[h] : 1.0f;
-  for (int idx = tid; idx < live * (kHeadDim / 2); idx += 256) {
-    const int row = idx / (kHeadDim / 2), ch = 2 * (idx - row * (kHeadDim / 2));
-    float M = kNegInf, L = 0.0f, o[2] = {0.0f, 0.0f};
 #pragma unroll
-    for (int w = 0; w < 4; ++w) M = fmaxf(M, s_m[w * live + row]);
+  for (int r = 0; r < RT; ++r) {
+    const int row = 16 * r + (tid >> 4), c = tid & 15;
+    if (row >= live) break;
+    const mf32x4 m = *(const mf32x4*)(s_m + 4 * row), l = *(const mf32x4*)(s_l + 4 * row);
+    const float M = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+    float L = 0.0f;
+    MaskedPairs o{};
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
-      const float m = s_m[w * live + row], a = m == kNegInf ? (s_l[w * live + row] == 0.0f ? 0.0f : 1.0f) : fast_exp2(m - M);
-      const float* src = s_o + (w * live + row) * kMaskedRowPad + ch;
-      if (a != 0.0f) {
-        L = fmaf(a, s_l[w * live + row], L);
-        o[0] = fmaf(a, src[0], o[0]), o[1] = fmaf(a, src[1], o[1]);
+      // Waves that saw nothing have no maximum, nor have those whose scores were all NaN, whose sums carry that on.
+      const float a = m[w] == kNegInf ? (l[w] == 0.0f ? 0.0f : 1.0f) : fast_exp2(m[w] - M);
+      const float* src = s_o + (w * live + row) * kMaskedRowPad + 2 * c;
+      if (a != 0.0f) L = fmaf(a, l[w], L);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 x = *(const float2*)(src + 32 * i);
+        if (a != 0.0f) o.x[i][0] = fmaf(a, x.x, o.x[i][0]), o.x[i][1] = fmaf(a, x.y, o.x[i][1]);
       }
     }
-    const float inv = L == 0.0f ? 0.0f : vscale / L;
-    o[0] *= inv, o[1] *= inv;
+    const float inv = L == 0.0f ? 0.0f : vscale * __builtin_amdgcn_rcpf(L);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o.x[i][0] *= inv, o.x[i][1] *= inv;
     const float lse2 = L == 0.0f ? kNegInf : (M == kNegInf ? 0.0f : M) + __log2f(L);
-    if (pieces == 1) {
-      masked_write(p, b, h, row, ch, 2, o, lse2);
-    } else {
-      ws_store2(p.ws_out + (slot * p.live_rows + row) * kHeadDim + ch, o[0], o[1]);
-      if (ch == 0) ws_store(p.ws_lse + slot * p.live_rows + row, lse2);
-    }
+    if (pieces == 1) masked_store_pairs(p, b, h, row, c, o, lse2);
+    else masked_store_partial(p, slot, row, c, o, lse2);
   }
   if (pieces == 1) return;
   ws_publish();
@@ -707,14 +783,14 @@ __global__ __launch_bounds__(256, RT == 1 ? 3 : 2) void masked_few_kernel(const 
 
 // ---- many rows --------------------------------------------------------------------------------------------------
 
-constexpr int kMaskedItem = 8 * 64;                   // 16-byte units of one step's K or V operands in LDS
 constexpr int kMaskedChunk = 4 * kMaskedItem;         // two steps: K, K, V, V
 // Two chunks, their per-token scales, and the waves' weights of a careful pass.
 constexpr int kMaskedManyLds = 2 * kMaskedChunk * 16 + (2 * 2 * 64 + 4 * kMaskedStep * 16) * 4;
 static_assert(2 * (kMaskedManyLds + 64) <= 160 << 10, "two workgroups to a CU");
+static_assert(128 * (kMaskedRowPad + 1) * 4 <= kMaskedManyLds, "the rows fit where the operands lay");
 
 // The piece's steps t0 .. t1 - 1, two at a time, folded into each wave's rows (mine: what they see).
-template <int KV, int SK, bool QS, int RT, bool CAREFUL>
+template <int KV, int SK, bool PU, bool QS, int RT, bool CAREFUL>
 __device__ __forceinline__ void masked_many_steps(const MaskedParams& p, const MaskedRange& rg, const MaskedRange& mine, int b, int h,
                                                   int t0, int t1, int lane, int wave, bool idle, float qs,
                                                   const mu32x4 (&q)[RT][QS ? 8 : 4], mu32x4* s_op, float* s_scale,
@@ -723,24 +799,23 @@ __device__ __forceinline__ void masked_many_steps(const MaskedParams& p, const M
   masked_rows_reset(st);
   MaskedRaw<KV> raw;
   float sc = 0.0f;
+  int list = t0 < t1 ? masked_page_list<PU>(p, rg, b, t0 + my_step, 0, t1, lane) : 0;
   auto issue = [&](int t) {  // chunk at step t of the list; steps past the piece's last repeat it
     const int token0 = masked_token0(rg, min(t + my_step, t1 - 1));
-    const MaskedPages pages = masked_pages(p, b, token0, rg.len);
+    const MaskedPages pages = masked_pages(list);
+    list = masked_page_list<PU>(p, rg, b, t + 2 + my_step, 0, t1, lane);
     if (wave < 2) {
-      masked_issue_k<KV, false>(p, b, h, token0, rg.len, pages, lane, raw);
-      if constexpr (SK == kScaleTokenHead) sc = masked_issue_scale(p, b, h, token0, rg.len, pages, lane);
+      masked_issue_k<KV, PU, false>(p, b, h, token0, rg.len, pages, lane, raw);
+      if constexpr (SK == kScaleTokenHead) sc = masked_issue_scale<PU>(p, b, h, token0, rg.len, pages, lane);
     } else {
-      masked_issue_v<KV, false>(p, b, h, token0, rg.len, pages, lane, raw);
+      masked_issue_v<KV, PU, false>(p, b, h, token0, rg.len, pages, lane, raw);
     }
   };
   if (t0 < t1) issue(t0);
   for (int t = t0, buf = 0; t < t1; t += 2, buf ^= 1) {
-    mu32x4* dst = s_op + buf * kMaskedChunk + wave * kMaskedItem + lane;
+    mu32x4* dst = s_op + buf * kMaskedChunk + wave * kMaskedItem;
     if (wave < 2) {
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int s = 0; s < 4; ++s) dst[64 * (4 * u + s)] = masked_k_frag<KV>(raw, u, s);
+      masked_k_place<KV>(raw, lane, dst);
       if constexpr (SK == kScaleTokenHead) s_scale[(2 * buf + wave) * 64 + lane] = sc;
     } else {
 #pragma unroll
@@ -748,12 +823,12 @@ __device__ __forceinline__ void masked_many_steps(const MaskedParams& p, const M
         mu32x4 f[4];
         masked_v_frags<KV, CAREFUL>(raw, c4, f);
 #pragma unroll
-        for (int c = 0; c < 4; ++c) dst[64 * (4 * c4 + c)] = f[c];
+        for (int c = 0; c < 4; ++c) dst[64 * (4 * c4 + c) + lane] = f[c];
       }
     }
     __syncthreads();
     if (t + 2 < t1) issue(t + 2);
-    const mu32x4* src = s_op + buf * kMaskedChunk + lane;
+    const mu32x4* src = s_op + buf * kMaskedChunk;
 #pragma unroll
     for (int u2 = 0; u2 < 2; ++u2) {
       const int token0 = masked_token0(rg, min(t + u2, t1 - 1));
@@ -765,7 +840,7 @@ __device__ __forceinline__ void masked_many_steps(const MaskedParams& p, const M
       for (int u = 0; u < 2; ++u)
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
-          const mu32x4 f = src[u2 * kMaskedItem + 64 * (4 * u + s)];
+          const mu32x4 f = masked_k_frag<KV>(src + u2 * kMaskedItem, u, s, lane);
 #pragma unroll
           for (int r = 0; r < RT; ++r) {
             if constexpr (QS) S[r][u] = masked_mfma(f, q[r][4 + s], S[r][u]);
@@ -778,7 +853,7 @@ __device__ __forceinline__ void masked_many_steps(const MaskedParams& p, const M
                                           weights);
 #pragma unroll
       for (int c = 0; c < 8; ++c) {
-        const mu32x4 f = src[(2 + u2) * kMaskedItem + 64 * c];
+        const mu32x4 f = src[(2 + u2) * kMaskedItem + 64 * c + lane];
 #pragma unroll
         for (int r = 0; r < RT; ++r) {
           st.o[r][c] = masked_mfma(f, w[r][1], st.o[r][c]);
@@ -789,7 +864,7 @@ __device__ __forceinline__ void masked_many_steps(const MaskedParams& p, const M
   }
 }
 
-template <int KV, int SK, bool QS, int RT>
+template <int KV, int SK, bool PU, bool QS, int RT>
 __global__ __launch_bounds__(256, 2) void masked_many_kernel(const MaskedParams p) {
   extern __shared__ mu32x4 s_op[];  // [2 chunks][K0 K1 V0 V1][8 operands][64 lanes]
   __shared__ int s_last, s_bad;
@@ -819,36 +894,43 @@ __global__ __launch_bounds__(256, 2) void masked_many_kernel(const MaskedParams 
   masked_load_q<KV, QS, RT>(p, b, h, first, rows, lane, q);
   const float qs = masked_qscale<SK>(p, h);
 
-  masked_many_steps<KV, SK, QS, RT, false>(p, rg, mine, b, h, t0, t1, lane, wave, idle, qs, q, s_op, s_scale, st);
+  masked_many_steps<KV, SK, PU, QS, RT, false>(p, rg, mine, b, h, t0, t1, lane, wave, idle, qs, q, s_op, s_scale, st);
   if (tid == 0) s_bad = 0;
   __syncthreads();
   if (masked_nonfinite(st)) s_bad = 1;
   __syncthreads();
-  if (s_bad) masked_many_steps<KV, SK, QS, RT, true>(p, rg, mine, b, h, t0, t1, lane, wave, idle, qs, q, s_op, s_scale, st);
+  if (s_bad) masked_many_steps<KV, SK, PU, QS, RT, true>(p, rg, mine, b, h, t0, t1, lane, wave, idle, qs, q, s_op, s_scale, st);
 
+  // Rows go out through LDS (the operands' place), so that whole pieces of them are stored.
+  float* s_o = (float*)s_op;  // [BM][kMaskedRowPad], then each row's log2-sum-exp
+  float* s_lse = s_o + BM * kMaskedRowPad;
   const int64_t seg = ((int64_t)b * p.Hkv + h) * p.tiles + tile, slot = seg * p.max_pieces + piece;
   const float vscale = SK == kScaleHead ? p.vs[h] : 1.0f;
+  __syncthreads();  // the operands are read
 #pragma unroll
   for (int r = 0; r < RT; ++r) {
     const float l = sum_xor<32>(sum_xor<16>(st.l[r]));
     const int row = 16 * RT * wave + 16 * r + n;
-    if (row >= live) continue;
-    const float inv = l == 0.0f ? 0.0f : vscale / l;
-    const float lse2 = l == 0.0f ? kNegInf : (st.m[r] == kNegInf ? 0.0f : st.m[r]) + __log2f(l);
+    const float inv = l == 0.0f ? 0.0f : vscale * __builtin_amdgcn_rcpf(l);
+    if (g == 0) s_lse[row] = l == 0.0f ? kNegInf : (st.m[r] == kNegInf ? 0.0f : st.m[r]) + __log2f(l);
+    float* dst = s_o + row * kMaskedRowPad + 32 * g;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int c = 0; c < 8; c += 4)
+        *(mf32x4*)(dst + 8 * i + c) =
+            mf32x4{st.o[r][c][i] * inv, st.o[r][c + 1][i] * inv, st.o[r][c + 2][i] * inv, st.o[r][c + 3][i] * inv};
+  }
+  __syncthreads();
+  for (int row = tid >> 4; row < live; row += 16) {
+    MaskedPairs o;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      float o[8];
-#pragma unroll
-      for (int c = 0; c < 8; ++c) o[c] = st.o[r][c][i] * inv;
-      const int ch = 32 * g + 8 * i;
-      if (pieces == 1) {
-        masked_write(p, b, h, r0 + row, ch, 8, o, lse2);
-      } else {
-#pragma unroll
-        for (int c = 0; c < 8; c += 2) ws_store2(p.ws_out + (slot * p.live_rows + row) * kHeadDim + ch + c, o[c], o[c + 1]);
-        if (ch == 0) ws_store(p.ws_lse + slot * p.live_rows + row, lse2);
-      }
+      const float2 x = *(const float2*)(s_o + row * kMaskedRowPad + 2 * (tid & 15) + 32 * i);
+      o.x[i][0] = x.x, o.x[i][1] = x.y;
     }
+    if (pieces == 1) masked_store_pairs(p, b, h, r0 + row, tid & 15, o, s_lse[row]);
+    else masked_store_partial(p, slot, row, tid & 15, o, s_lse[row]);
   }
   if (pieces == 1) return;
   ws_publish();
@@ -862,30 +944,34 @@ __global__ __launch_bounds__(256, 2) void masked_many_kernel(const MaskedParams 
 
 // ---- launches ---------------------------------------------------------------------------------------------------
 
-template <int KV, int SK, bool QS>
+template <int KV, int SK, bool PU, bool QS>
 static hipError_t launch_masked_t(const MaskedParams& p, int rt, bool many, int grid, hipStream_t stream) {
   const int live = p.live_rows;
-  // The merge's rows, or the scales and weights that lie there before it.
+  // The merge's rows, or the operands, scales and weights that lie there before it.
   const size_t merge = (size_t)4 * live * (kMaskedRowPad + 2) * sizeof(float);
-  const size_t early = (size_t)(4 * 64 + 4 * kMaskedStep * 16) * sizeof(float);
+  const size_t early = (size_t)(4 * 4 * kMaskedItem + 4 * 64 + 4 * kMaskedStep * 16) * sizeof(float);
   const size_t few = merge > early ? merge : early;
-  const size_t lots = kMaskedManyLds;
-  const dim3 g(grid), t(256);
   hipError_t e = hipSuccess;
-  auto allow = [&](auto kernel, size_t bytes) {  // more than 64 KiB of dynamic LDS has to be asked for, once per device
-    if (bytes > (64u << 10)) e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
-    return e == hipSuccess;
+  auto run = [&](auto kernel, size_t lds) {
+    if (lds > (64u << 10))  // has to be asked for, once per device
+      e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+    if (e == hipSuccess) hipLaunchKernelGGL(kernel, dim3(grid), dim3(256), lds, stream, p);
   };
-  if (many && rt == 2) {
-    if (allow(masked_many_kernel<KV, SK, QS, 2>, lots)) hipLaunchKernelGGL((masked_many_kernel<KV, SK, QS, 2>), g, t, lots, stream, p);
-  } else if (many) {
-    if (allow(masked_many_kernel<KV, SK, QS, 1>, lots)) hipLaunchKernelGGL((masked_many_kernel<KV, SK, QS, 1>), g, t, lots, stream, p);
-  } else if (rt == 2) {
-    if (allow(masked_few_kernel<KV, SK, QS, 2>, few)) hipLaunchKernelGGL((masked_few_kernel<KV, SK, QS, 2>), g, t, few, stream, p);
-  } else {
-    if (allow(masked_few_kernel<KV, SK, QS, 1>, few)) hipLaunchKernelGGL((masked_few_kernel<KV, SK, QS, 1>), g, t, few, stream, p);
-  }
+  if (many && rt == 2) run(masked_many_kernel<KV, SK, PU, QS, 2>, kMaskedManyLds);
+  else if (many) run(masked_many_kernel<KV, SK, PU, QS, 1>, kMaskedManyLds);
+  else if (rt == 2) run(masked_few_kernel<KV, SK, PU, QS, 2>, few);
+  else run(masked_few_kernel<KV, SK, PU, QS, 1>, few);
   return e == hipSuccess ? hipGetLastError() : e;
+}
+
+// PU: pages of at least 16 tokens, so that the 16 tokens of a group lie in one, whose id the whole wave reads.
+template <int KV, int SK>
+static hipError_t launch_masked(const MaskedParams& p, bool q_split, int rt, bool many, int grid, hipStream_t stream) {
+  if (p.logP >= 4)
+    return q_split ? launch_masked_t<KV, SK, true, true>(p, rt, many, grid, stream)
+                   : launch_masked_t<KV, SK, true, false>(p, rt, many, grid, stream);
+  return q_split ? launch_masked_t<KV, SK, false, true>(p, rt, many, grid, stream)
+                 : launch_masked_t<KV, SK, false, false>(p, rt, many, grid, stream);
 }
 
 }  // namespace bpt

@@ -4,8 +4,7 @@
 namespace bpt {
 
 hipError_t launch_masked_bf16(const MaskedParams& p, bool q_split, int rt, bool many, int grid, hipStream_t stream) {
-  return q_split ? launch_masked_t<kKvBf16, kScaleNone, true>(p, rt, many, grid, stream)
-                 : launch_masked_t<kKvBf16, kScaleNone, false>(p, rt, many, grid, stream);
+  return launch_masked<kKvBf16, kScaleNone>(p, q_split, rt, many, grid, stream);
 }
 
 }  // namespace bpt

@@ -4,8 +4,7 @@
 namespace bpt {
 
 hipError_t launch_masked_fp8_token(const MaskedParams& p, bool q_split, int rt, bool many, int grid, hipStream_t stream) {
-  return q_split ? launch_masked_t<kKvFp8, kScaleTokenHead, true>(p, rt, many, grid, stream)
-                 : launch_masked_t<kKvFp8, kScaleTokenHead, false>(p, rt, many, grid, stream);
+  return launch_masked<kKvFp8, kScaleTokenHead>(p, q_split, rt, many, grid, stream);
 }
 
 }  // namespace bpt

@@ -4,8 +4,7 @@
 namespace bpt {
 
 hipError_t launch_masked_int8_head(const MaskedParams& p, bool q_split, int rt, bool many, int grid, hipStream_t stream) {
-  return q_split ? launch_masked_t<kKvInt8, kScaleHead, true>(p, rt, many, grid, stream)
-                 : launch_masked_t<kKvInt8, kScaleHead, false>(p, rt, many, grid, stream);
+  return launch_masked<kKvInt8, kScaleHead>(p, q_split, rt, many, grid, stream);
 }
 
 }  // namespace bpt

@@ -374,7 +374,7 @@ struct MaskedParams {
   float* ws_out;       // [segments, max_pieces, live_rows, D] normalized partials
   float* ws_lse;       // [segments, max_pieces, live_rows] their log2-sum-exp
   unsigned* counters;  // [segments] arrivals; zero between calls
-  int B, Q, Hq, Hkv, G, P, logP, num_blocks, len_cap, table_i64, out_dtype;
+  int B, Q, Hq, Hkv, G, P, logP, num_blocks, max_blocks, len_cap, table_i64, out_dtype;
   int window;      // 0: none
   int max_prefix;  // prefix lengths above it are cut to it
   int tiles;       // row tiles of a KV head

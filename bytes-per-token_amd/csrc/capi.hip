@@ -1014,6 +1014,8 @@ int masked_setup(const bpt_decode_args* a, const bpt_mask_args* m, const char* f
   const int eb = a->kv_dtype == BPT_KV_BF16 ? 2 : 1;
   if (a->kv_stride_token < 0 || a->kv_stride_token * eb >= (int64_t(1) << 27))
     return fail(BPT_ERR_INVALID_ARGUMENT, "%s: 16 tokens of a page must lie within 2 GiB", fn);
+  if (a->scale_kind == BPT_SCALE_PER_TOKEN_HEAD && (a->scale_stride_token < 0 || a->scale_stride_token >= (int64_t(1) << 27)))
+    return fail(BPT_ERR_INVALID_ARGUMENT, "%s: the scales of 16 tokens must lie within 2^31 elements", fn);
 
   bpt::MaskedParams p{};
   p.B = a->batch;
@@ -1024,6 +1026,7 @@ int masked_setup(const bpt_decode_args* a, const bpt_mask_args* m, const char* f
   p.P = a->page_size;
   p.logP = log2i(a->page_size);
   p.num_blocks = a->num_blocks;
+  p.max_blocks = a->max_blocks_per_seq;
   const int64_t reach = (int64_t)a->max_blocks_per_seq * a->page_size;
   p.len_cap = (int)std::min<int64_t>(a->max_context, reach);
   p.window = m->window >= p.len_cap ? 0 : m->window;  // a window of all tokens hides none
@@ -1034,12 +1037,14 @@ int masked_setup(const bpt_decode_args* a, const bpt_mask_args* m, const char* f
   if (!std::isfinite(p.qscale) || !std::isfinite(2.0f * p.cap))
     return fail(BPT_ERR_INVALID_ARGUMENT, "%s: sm_scale %g and softcap %g are out of range", fn, a->sm_scale, m->softcap);
 
-  // Rows: one wave holds up to 32 (it reads its tokens' keys and values straight into registers), else four waves share
-  // tiles of 64 or 128 whose operands they convert once between them.
+  // Few rows: tiles of 16, whose waves read their tokens' keys and values straight into registers (up to three tiles read them
+  // again, from L2). Many: four waves share tiles of 64 or 128 whose operands they convert once between them. In a graph, us, 16
+  // sequences, three tiles of 16 against one of 64: FP8 48 rows x 128 / 600 / 3000 tokens 6.7 : 10.3, 19.2 : 24.7, 43.3 : 52.2,
+  // BF16 7.2 : 11.9, 23.6 : 26.6, 61.5 : 60.5.
   const int rows = pl.rows;
-  plan->many = rows > 32;
-  plan->rt = plan->many ? (rows > 64 ? 2 : 1) : (rows > 16 ? 2 : 1);
-  const int tile = plan->many ? 64 * plan->rt : rows;
+  plan->many = rows > 48;
+  plan->rt = rows > 64 ? 2 : 1;
+  const int tile = plan->many ? 64 * plan->rt : 16;
   if ((int64_t)rows * p.G > 0x7fffffffLL)  // row / G is exact below that
     return fail(BPT_ERR_INVALID_ARGUMENT, "%s: too many rows", fn);
   p.G_inv = (unsigned)((((uint64_t)1 << 32) + p.G - 1) / p.G);
@@ -1061,7 +1066,7 @@ int masked_setup(const bpt_decode_args* a, const bpt_mask_args* m, const char* f
   p.max_pieces = (int)std::max<int64_t>(1, (steps + p.piece - 1) / p.piece);
   const int64_t slots = segments * p.max_pieces;
   if (slots > 0x70000000LL) return fail(BPT_ERR_INVALID_ARGUMENT, "%s: batch x heads x rows too large", fn);
-  plan->grid = (int)(plan->many ? slots : ((int64_t)a->batch * p.max_pieces + 7) / 8 * 8 * p.Hkv);  // few rows: see the kernel
+  plan->grid = (int)(plan->many ? slots : ((int64_t)a->batch * p.max_pieces + 7) / 8 * 8 * p.Hkv * p.tiles);  // few rows: see the kernel
   plan->ws_out_floats = p.max_pieces > 1 ? (size_t)slots * p.live_rows * a->head_dim : 0;
   plan->workspace = p.max_pieces > 1 ? align256((plan->ws_out_floats + (size_t)slots * p.live_rows) * sizeof(float)) : 0;
   plan->counters = p.max_pieces > 1 ? align256((size_t)segments * sizeof(unsigned)) : 0;

@@ -22,8 +22,8 @@
 // before them. The pieces of a tile meet in float32 partials, which the last workgroup to arrive combines in order.
 //
 // Two kernels:
-//  * few rows (up to 32 of a KV head): the waves of a workgroup take steps in turn, straight from memory into registers,
-//    and merge through LDS at the end. Bound by the cache's bytes.
+//  * few rows (up to 48 of a KV head, in tiles of 16): the waves of a workgroup take steps in turn, straight from memory into
+//    registers, and merge through LDS at the end. Bound by the cache's bytes, short calls by the latency of a piece.
 //  * many rows: a workgroup's four waves hold 64 or 128 rows; each of two steps' keys and values is loaded and converted by
 //    one wave and read by all from LDS, where operands lie in the order lanes take them (no bank conflicts, no swizzle).
 //    Bound by the vector units (the scores' exponentials).
@@ -57,10 +57,9 @@ __device__ __forceinline__ uint32_t masked_fp8_pair(uint32_t w, bool high) {
 }
 // Four int8 codes -> bf16, through float32 (exact).
 __device__ __forceinline__ mu32x2 masked_int8x4(uint32_t w) {
-  const uint32_t u = w ^ 0x80808080u;
   float f[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) f[i] = (float)((u >> (8 * i)) & 0xffu) - 128.0f;
+  for (int i = 0; i < 4; ++i) f[i] = (float)(int8_t)((w >> (8 * i)) & 0xffu);
   return mu32x2{__builtin_amdgcn_perm(__float_as_uint(f[1]), __float_as_uint(f[0]), 0x07060302u),
                 __builtin_amdgcn_perm(__float_as_uint(f[3]), __float_as_uint(f[2]), 0x07060302u)};
 }
@@ -114,11 +113,28 @@ __device__ __forceinline__ int64_t masked_row(const MaskedParams& p, int b, int 
   const int e = masked_clamp_page(p, ((const int32_t*)p.table)[((int64_t)b * p.table_sb + (tok >> p.logP)) << p.table_i64]);
   return (int64_t)e * p.kv_sblk + (int64_t)(tok & (p.P - 1)) * p.kv_stok + (int64_t)h * p.kv_shead;
 }
-// The 16-token group's base offset and the last of its rows that may be read.
-__device__ __forceinline__ int64_t masked_group(const MaskedParams& p, int h, int e, int token, int len, int& rmax) {
-  rmax = max(len - 1 - token, 0);
-  return (int64_t)masked_clamp_page(p, sread(e)) * p.kv_sblk + (int64_t)(min(token, len - 1) & (p.P - 1)) * p.kv_stok +
-         (int64_t)h * p.kv_shead;
+// Where a step's two 16-token groups lie (pages of at least 16 tokens): byte offsets of their first rows, and from there of the
+// last row that holds a token of the sequence, up to which the others are cut. A group behind the sequence reads the first one.
+struct MaskedSpot {
+  int64_t base[2];
+  uint32_t last[2];
+  int page[2], rows[2];  // the page, and the last row's number
+};
+template <bool PU>
+__device__ __forceinline__ MaskedSpot masked_spot(const MaskedParams& p, int h, MaskedPages pages, int token0, int len) {
+  MaskedSpot s{};
+  if constexpr (PU) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const bool in = token0 + 16 * t < len;
+      const int token = in ? token0 + 16 * t : token0;
+      s.page[t] = masked_clamp_page(p, in ? pages.e[t] : pages.e[0]);
+      s.rows[t] = min(len - 1 - token, 15);
+      s.base[t] = (int64_t)s.page[t] * p.kv_sblk + (int64_t)(token & (p.P - 1)) * p.kv_stok + (int64_t)h * p.kv_shead;
+      s.last[t] = (uint32_t)s.rows[t] * (uint32_t)p.kv_stok;
+    }
+  }
+  return s;
 }
 
 // ONCE: read by this workgroup alone (past the caches), else by the other tiles of the head too.
@@ -131,52 +147,60 @@ __device__ __forceinline__ void masked_load(const uint8_t* src, uint32_t* w) {
 }
 
 // Keys: whole rows, 16 bytes a lane (of codes, 8 lanes to a token and 8 tokens to a load; of bf16, 16 and 4), which the memory
-// pipeline serves faster than the operands' own order. They get into that order through LDS (masked_k_place).
+// pipeline serves faster than the operands' own order. They get into that order through LDS.
 template <int KV, bool PU, bool ONCE>
-__device__ __forceinline__ void masked_issue_k(const MaskedParams& p, int b, int h, int token0, int len, MaskedPages pages,
-                                               int lane, MaskedRaw<KV>& r) {
+__device__ __forceinline__ void masked_issue_k(const MaskedParams& p, int b, int h, int token0, int len, const MaskedSpot& s, int lane,
+                                               MaskedRaw<KV>& r) {
   constexpr int S = KV == kKvBf16 ? 16 : 8, PER = 64 / S;  // 16-byte segments of a row, rows of a load
-  const int row = lane / S, seg = lane % S;
+  const int row = lane / S;
+  const uint32_t x = 16 * (lane % S), stok = (uint32_t)p.kv_stok;
 #pragma unroll
   for (int t = 0; t < 2; ++t) {
-    int rmax = 0;
-    const int64_t base = PU ? masked_group(p, h, pages.e[t], token0 + 16 * t, len, rmax) : 0;
+    const uint32_t last = s.last[t] + x;
 #pragma unroll
     for (int j = 0; j < 16 / PER; ++j) {
-      const uint8_t* src = PU ? p.k + base + (uint32_t)(min(PER * j + row, rmax) * (uint32_t)p.kv_stok + 16 * seg)
-                                       : p.k + masked_row(p, b, h, token0 + 16 * t + PER * j + row, len) + 16 * seg;
+      const uint8_t* src = PU ? p.k + s.base[t] + min((uint32_t)(PER * j + row) * stok + x, last)
+                              : p.k + masked_row(p, b, h, token0 + 16 * t + PER * j + row, len) + x;
       masked_load<4, ONCE>(src, r.w + 4 * (16 / PER * t + j));
     }
   }
 }
 // Values: lane (n, g) takes channels 8 n .. + 7 of tokens 4 g + i and 16 + 4 g + i.
 template <int KV, bool PU, bool ONCE>
-__device__ __forceinline__ void masked_issue_v(const MaskedParams& p, int b, int h, int token0, int len, MaskedPages pages,
-                                               int lane, MaskedRaw<KV>& r) {
+__device__ __forceinline__ void masked_issue_v(const MaskedParams& p, int b, int h, int token0, int len, const MaskedSpot& s, int lane,
+                                               MaskedRaw<KV>& r) {
   constexpr int W = KV == kKvBf16 ? 4 : 2;
-  const int n = lane & 15, g = lane >> 4;
+  const int g = lane >> 4;
+  const uint32_t x = 4 * W * (lane & 15), stok = (uint32_t)p.kv_stok;
 #pragma unroll
   for (int t = 0; t < 2; ++t) {
-    int rmax = 0;
-    const int64_t base = PU ? masked_group(p, h, pages.e[t], token0 + 16 * t, len, rmax) : 0;
+    const uint32_t last = s.last[t] + x;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const uint8_t* src = PU ? p.v + base + (uint32_t)(min(4 * g + i, rmax) * (uint32_t)p.kv_stok + 4 * W * n)
-                                       : p.v + masked_row(p, b, h, token0 + 16 * t + 4 * g + i, len) + 4 * W * n;
+      const uint8_t* src = PU ? p.v + s.base[t] + min((uint32_t)(4 * g + i) * stok + x, last)
+                              : p.v + masked_row(p, b, h, token0 + 16 * t + 4 * g + i, len) + x;
       masked_load<W, ONCE>(src, r.w + W * (4 * t + i));
     }
   }
 }
 // Per-token scales: lane l < 32 takes the key's scale of token l, the others the value's of token l - 32.
 template <bool PU>
-__device__ __forceinline__ float masked_issue_scale(const MaskedParams& p, int b, int h, int token0, int len, MaskedPages pages,
+__device__ __forceinline__ float masked_issue_scale(const MaskedParams& p, int b, int h, int token0, int len, const MaskedSpot& s,
                                                     int lane) {
-  const int tok = min(token0 + (lane & 31), len - 1);
-  int e;
-  if (PU) e = (lane & 16) ? pages.e[1] : pages.e[0];
-  else e = ((const int32_t*)p.table)[((int64_t)b * p.table_sb + (tok >> p.logP)) << p.table_i64];
-  return (lane < 32 ? p.ks : p.vs)[(int64_t)masked_clamp_page(p, e) * p.sc_sblk + (int64_t)(tok & (p.P - 1)) * p.sc_stok +
-                                   (int64_t)h * p.sc_shead];
+  const float* src = lane < 32 ? p.ks : p.vs;
+  if constexpr (PU) {
+    int64_t base[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+      base[t] = (int64_t)s.page[t] * p.sc_sblk + (int64_t)((token0 + 16 * t < len ? token0 + 16 * t : token0) & (p.P - 1)) * p.sc_stok +
+                (int64_t)h * p.sc_shead;
+    const int row = min(lane & 15, (lane & 16) ? s.rows[1] : s.rows[0]);
+    return src[((lane & 16) ? base[1] : base[0]) + (uint32_t)row * (uint32_t)p.sc_stok];
+  } else {
+    const int tok = min(token0 + (lane & 31), len - 1);
+    const int e = ((const int32_t*)p.table)[((int64_t)b * p.table_sb + (tok >> p.logP)) << p.table_i64];
+    return src[(int64_t)masked_clamp_page(p, e) * p.sc_sblk + (int64_t)(tok & (p.P - 1)) * p.sc_stok + (int64_t)h * p.sc_shead];
+  }
 }
 
 // Loaded key rows into LDS as the first product's operands: operand s of 16-token group t is 64 units of 16 bytes, unit 16 g + n
@@ -208,6 +232,24 @@ template <int KV>
 __device__ __forceinline__ mu32x4 masked_k_frag(const mu32x4* src, int t, int s, int lane) {
   return src[masked_k_unit(t, s, lane >> 4, lane & 15, KV == kKvBf16 ? s & 1 : s >> 1)];
 }
+// The same within one wave, which converts after reading: rows as loaded, segments permuted within their eights by row (the 8 lanes
+// that store a row's segments, and the 8 that read one segment of 8 rows, touch all banks).
+template <int KV>
+__device__ __forceinline__ void masked_k_keep(const MaskedRaw<KV>& r, int lane, mu32x4* tile) {
+  constexpr int S = KV == kKvBf16 ? 16 : 8, PER = 64 / S;
+#pragma unroll
+  for (int j = 0; j < 32 / PER; ++j) {
+    const int row = PER * j + lane / S;
+    tile[S * row + ((lane % S) ^ (row & 7))] = mu32x4{r.w[4 * j], r.w[4 * j + 1], r.w[4 * j + 2], r.w[4 * j + 3]};
+  }
+}
+// Segment c of the lane's operands: of bf16 those of product c, of codes those of products 2 c and 2 c + 1.
+template <int KV>
+__device__ __forceinline__ mu32x4 masked_k_take(const mu32x4* tile, int t, int c, int lane) {
+  const int n = lane & 15, g = lane >> 4;
+  return tile[(KV == kKvBf16 ? 16 : 8) * (16 * t + n) + ((4 * c + g) ^ (n & 7))];
+}
+
 // The value operands of four channel blocks c = 4 q .. 4 q + 3: channel 8 n + c of the lane's 8 tokens. CAREFUL: with values
 // that are not finite replaced by zeros.
 template <int KV, bool CAREFUL>
@@ -268,6 +310,9 @@ __device__ __forceinline__ MaskedPages masked_pages(int list, int which = 0) {
   return MaskedPages{{__builtin_amdgcn_readlane(list, 2 * which), __builtin_amdgcn_readlane(list, 2 * which + 1)}};
 }
 
+// Row r's query, r / G by a multiplication (the host checks that it is exact).
+__device__ __forceinline__ int masked_query(const MaskedParams& p, int r) { return p.G == 1 ? r : (int)__umulhi((unsigned)r, p.G_inv); }
+
 __device__ __forceinline__ void masked_bounds(const MaskedParams& p, int b, int qi, int len, int& pos, int& lo, int& hi) {
   pos = len - p.Q + qi;
   lo = p.window > 0 ? max(pos - p.window + 1, 0) : 0;
@@ -279,7 +324,7 @@ __device__ __forceinline__ void masked_bounds(const MaskedParams& p, int b, int 
 // Lowest / highest bounds over rows r0 .. r1 - 1 of a KV head, the same in every lane.
 __device__ __forceinline__ void masked_extent(const MaskedParams& p, int b, int r0, int r1, int lane, MaskedRange& r) {
   r.min_lo = 0x7fffffff, r.max_lo = 0, r.min_hi = 0x7fffffff, r.max_hi = 0;
-  const int q0 = r0 / p.G, q1 = (r1 - 1) / p.G;
+  const int q0 = masked_query(p, r0), q1 = masked_query(p, r1 - 1);
   int pos, lo, hi;
   const bool scan = p.starts != nullptr;  // else both bounds rise with the query: the first and the last one tell
   for (int q = scan ? q0 + lane : q0; q <= q1; q += scan ? 64 : max(q1 - q0, 1)) {
@@ -320,9 +365,6 @@ __device__ __forceinline__ bool masked_whole(const MaskedRange& r, int token0) {
 __device__ __forceinline__ bool masked_unseen(const MaskedRange& r, int token0) {
   return token0 >= r.prefix && (token0 >= r.max_hi || token0 + kMaskedStep <= r.min_lo);
 }
-
-// Row r's query, r / G by a multiplication (the host checks that it is exact).
-__device__ __forceinline__ int masked_query(const MaskedParams& p, int r) { return p.G == 1 ? r : (int)__umulhi((unsigned)r, p.G_inv); }
 
 template <int RT>
 __device__ __forceinline__ void masked_rows_init(const MaskedParams& p, int b, int h, int first, int rows, int len, int lane,
@@ -618,68 +660,72 @@ __device__ __forceinline__ int masked_index() {
   return k * q + min(k, r) + (x >> 3);
 }
 
+constexpr int masked_key_units(int kv) { return kMaskedStep * (kv == kKvBf16 ? 16 : 8); }  // 16-byte units of a step's key rows
+
 // ---- few rows ---------------------------------------------------------------------------------------------------
 
-// One wave's steps t, t + 4, ... < t1 folded into its rows. The next step's keys are requested once this one's have gone to LDS,
+// One wave's steps t, t + 4, ... < t1 folded into its rows (list: the page ids of the first two). The next step's keys are requested once this one's have gone to LDS,
 // its values once this one's are multiplied, and the page ids of the step after that in between: no request stands behind a
 // branch, so that each is waited for by itself.
-template <int KV, int SK, bool PU, bool QS, int RT, bool CAREFUL>
+template <int KV, int SK, bool PU, bool QS, bool ONCE, bool CAREFUL>
 __device__ __forceinline__ void masked_few_steps(const MaskedParams& p, const MaskedRange& rg, int b, int h, int t, int t1, int lane,
-                                                 float qs, const mu32x4 (&q)[RT][QS ? 8 : 4], mu32x4* w_keys, float* w_scale,
-                                                 float* w_weights, MaskedRows<RT>& st) {
+                                                 float qs, const mu32x4 (&q)[1][QS ? 8 : 4], int list, mu32x4* w_keys,
+                                                 float* w_scale, float* w_weights, MaskedRows<1>& st) {
   masked_rows_reset(st);
   if (t >= t1) return;
   MaskedRaw<KV> k, v;
   float sc = 0.0f;
   int token0 = masked_token0(rg, t);
-  int list = masked_page_list<PU>(p, rg, b, t, 4, t1, lane);
   MaskedPages pages = masked_pages(list, 1);  // the next step's
   {
-    const MaskedPages pages = masked_pages(list);
-    masked_issue_k<KV, PU, true>(p, b, h, token0, rg.len, pages, lane, k);
-    if constexpr (SK == kScaleTokenHead) sc = masked_issue_scale<PU>(p, b, h, token0, rg.len, pages, lane);
-    masked_issue_v<KV, PU, true>(p, b, h, token0, rg.len, pages, lane, v);
+    const MaskedSpot spot = masked_spot<PU>(p, h, masked_pages(list), token0, rg.len);
+    masked_issue_k<KV, PU, ONCE>(p, b, h, token0, rg.len, spot, lane, k);
+    if constexpr (SK == kScaleTokenHead) sc = masked_issue_scale<PU>(p, b, h, token0, rg.len, spot, lane);
+    masked_issue_v<KV, PU, ONCE>(p, b, h, token0, rg.len, spot, lane, v);
   }
   auto step = [&](auto last) {
-    masked_k_place<KV>(k, lane, w_keys);
+    masked_k_keep<KV>(k, lane, w_keys);
     if constexpr (SK == kScaleTokenHead) w_scale[lane] = sc;
     const int next = last ? 0 : masked_token0(rg, t + 4);
+    MaskedSpot spot{};
     if constexpr (!last) {
-      masked_issue_k<KV, PU, true>(p, b, h, next, rg.len, pages, lane, k);
-      if constexpr (SK == kScaleTokenHead) sc = masked_issue_scale<PU>(p, b, h, next, rg.len, pages, lane);
+      spot = masked_spot<PU>(p, h, pages, next, rg.len);
+      masked_issue_k<KV, PU, ONCE>(p, b, h, next, rg.len, spot, lane, k);
+      if constexpr (SK == kScaleTokenHead) sc = masked_issue_scale<PU>(p, b, h, next, rg.len, spot, lane);
       list = masked_page_list<PU>(p, rg, b, t + 8, 0, t1, lane);
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // the wave's lanes read one another's
-    mf32x4 S[RT][2];
+    mf32x4 S[1][2] = {{mf32x4{0.0f, 0.0f, 0.0f, 0.0f}, mf32x4{0.0f, 0.0f, 0.0f, 0.0f}}};
+    constexpr int C = KV == kKvBf16 ? 4 : 2;  // segments of a lane, each for 4 / C products
+    mu32x4 seg[2][C];
 #pragma unroll
-    for (int r = 0; r < RT; ++r) S[r][0] = S[r][1] = mf32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int c = 0; c < C; ++c) seg[u][c] = masked_k_take<KV>(w_keys, u, c, lane);
 #pragma unroll
     for (int u = 0; u < 2; ++u)
 #pragma unroll
       for (int s = 0; s < 4; ++s) {
-        const mu32x4 f = masked_k_frag<KV>(w_keys, u, s, lane);
-#pragma unroll
-        for (int r = 0; r < RT; ++r) {
-          if constexpr (QS) S[r][u] = masked_mfma(f, q[r][4 + s], S[r][u]);
-          S[r][u] = masked_mfma(f, q[r][s], S[r][u]);
-        }
+        mu32x4 f;
+        if constexpr (KV == kKvBf16) f = seg[u][s];
+        else f = masked_codes8<KV>(seg[u][s >> 1][2 * (s & 1)], seg[u][s >> 1][2 * (s & 1) + 1]);
+        if constexpr (QS) S[0][u] = masked_mfma(f, q[0][4 + s], S[0][u]);
+        S[0][u] = masked_mfma(f, q[0][s], S[0][u]);
       }
-    mu32x4 w[RT][2];
-    masked_softmax<KV, SK, RT, CAREFUL>(p, rg, b, h, token0, masked_whole(rg, token0), lane, qs, w_scale, S, st, w, w_weights);
+    mu32x4 w[1][2];
+    masked_softmax<KV, SK, 1, CAREFUL>(p, rg, b, h, token0, masked_whole(rg, token0), lane, qs, w_scale, S, st, w, w_weights);
 #pragma unroll
     for (int c4 = 0; c4 < 2; ++c4) {
       mu32x4 f[4];
       masked_v_frags<KV, CAREFUL>(v, c4, f);
 #pragma unroll
-      for (int c = 0; c < 4; ++c)
-#pragma unroll
-        for (int r = 0; r < RT; ++r) {
-          st.o[r][4 * c4 + c] = masked_mfma(f[c], w[r][1], st.o[r][4 * c4 + c]);
-          st.o[r][4 * c4 + c] = masked_mfma(f[c], w[r][0], st.o[r][4 * c4 + c]);
-        }
+      for (int c = 0; c < 4; ++c) {
+        st.o[0][4 * c4 + c] = masked_mfma(f[c], w[0][1], st.o[0][4 * c4 + c]);
+        st.o[0][4 * c4 + c] = masked_mfma(f[c], w[0][0], st.o[0][4 * c4 + c]);
+      }
     }
     if constexpr (!last) {
-      masked_issue_v<KV, PU, true>(p, b, h, next, rg.len, pages, lane, v);
+      masked_issue_v<KV, PU, ONCE>(p, b, h, next, rg.len, spot, lane, v);
       pages = masked_pages(list);
       token0 = next;
     }
@@ -688,8 +734,8 @@ __device__ __forceinline__ void masked_few_steps(const MaskedParams& p, const Ma
   step(std::true_type{});
 }
 
-template <int KV, int SK, bool PU, bool QS, int RT>
-__global__ __launch_bounds__(256, RT == 1 ? 3 : 2) void masked_few_kernel(const MaskedParams p) {
+template <int KV, int SK, bool PU, bool QS, bool ONCE>
+__global__ __launch_bounds__(256, KV == kKvBf16 ? 2 : 3) void masked_few_kernel(const MaskedParams p) {
   // [4 waves][live][kMaskedRowPad], then [live][4] m and l; on the way there key operands, scales and weights. Vectors, so that it
   // lies on a 16-byte boundary whatever other LDS there is: 16-byte accesses off it take eight times as long.
   extern __shared__ mf32x4 s_dyn[];
@@ -699,55 +745,57 @@ __global__ __launch_bounds__(256, RT == 1 ? 3 : 2) void masked_few_kernel(const 
   const int n = lane & 15, g = lane >> 4;
   // Workgroups go to the 8 XCDs in turn: the heads of a piece, whose rows share pages and lines of scales, go to one, and the
   // pieces are dealt out to the XCDs in turn, the first ones of all sequences before the second ones.
-  const int turn = (blockIdx.x >> 3) / p.Hkv * 8 + (blockIdx.x & 7), h = (blockIdx.x >> 3) % p.Hkv;
+  const int heads = p.Hkv * p.tiles, ht = (blockIdx.x >> 3) % heads;
+  const int turn = (blockIdx.x >> 3) / heads * 8 + (blockIdx.x & 7), h = ht / p.tiles, tile = ht - h * p.tiles;
   const int piece = turn / p.B, b = turn % p.B;
   if (piece >= p.max_pieces) return;
-  const int rows = p.Q * p.G;
-  const MaskedRange rg = masked_range(p, b, 0, rows, lane);
+  const int rows = p.Q * p.G, r0 = 16 * tile, live = min(rows - r0, 16), t0 = piece * p.piece;
+  mu32x4 q[1][QS ? 8 : 4];
+  masked_load_q<KV, QS, 1>(p, b, h, r0, rows, lane, q);
+  // Where steps follow one another from the sequence's first token on, the first page ids are known ahead of its length.
+  const bool plain = PU && p.window == 0 && !p.starts;
+  int list = 0;
+  if (plain) {
+    const int group = 2 * (t0 + wave + (lane & 2 ? 4 : 0)) + (lane & 1);
+    list = ((const int32_t*)p.table)[((int64_t)b * p.table_sb + min(group >> (p.logP - 4), p.max_blocks - 1)) << p.table_i64];
+  }
+  const MaskedRange rg = masked_range(p, b, r0, r0 + live, lane);
   const int pieces = max((rg.n + p.piece - 1) / p.piece, 1);
   if (piece >= pieces) return;
-  const int t0 = piece * p.piece, t1 = min(t0 + p.piece, rg.n);
-  const int live = rows;
+  const int t1 = min(t0 + p.piece, rg.n);
+  if (!plain && t0 + wave < t1) list = masked_page_list<PU>(p, rg, b, t0 + wave, 4, t1, lane);
+  const float vscale = SK == kScaleHead ? p.vs[h] : 1.0f, qs = masked_qscale<SK>(p, h);
 
-  MaskedRows<RT> st;
-  masked_rows_init<RT>(p, b, h, 0, rows, rg.len, lane, st);
-  mu32x4 q[RT][QS ? 8 : 4];
-  masked_load_q<KV, QS, RT>(p, b, h, 0, rows, lane, q);
-  const float qs = masked_qscale<SK>(p, h);
-  mu32x4* w_keys = (mu32x4*)smem + wave * kMaskedItem;  // this wave's key operands,
-  float* w_scale = smem + 4 * 4 * kMaskedItem + wave * 64;  // per-token scales
-  float* w_weights = smem + 4 * 4 * kMaskedItem + 4 * 64 + wave * kMaskedStep * 16;  // and, where needed, weights
-
-  masked_few_steps<KV, SK, PU, QS, RT, false>(p, rg, b, h, t0 + wave, t1, lane, qs, q, w_keys, w_scale, w_weights, st);
-  if (__any(masked_nonfinite(st)))
-    masked_few_steps<KV, SK, PU, QS, RT, true>(p, rg, b, h, t0 + wave, t1, lane, qs, q, w_keys, w_scale, w_weights, st);
+  MaskedRows<1> st;
+  masked_rows_init<1>(p, b, h, r0, rows, rg.len, lane, st);
+  mu32x4* w_keys = (mu32x4*)smem + wave * masked_key_units(KV);  // this wave's key rows,
+  float* w_scale = smem + 16 * masked_key_units(KV) + wave * 64;  // per-token scales
+  float* w_weights = smem + 16 * masked_key_units(KV) + 4 * 64 + wave * kMaskedStep * 16;  // and, where needed, weights
+  masked_few_steps<KV, SK, PU, QS, ONCE, false>(p, rg, b, h, t0 + wave, t1, lane, qs, q, list, w_keys, w_scale, w_weights, st);
+  if (__any(masked_nonfinite(st))) {
+    if (t0 + wave < t1) list = masked_page_list<PU>(p, rg, b, t0 + wave, 4, t1, lane);
+    masked_few_steps<KV, SK, PU, QS, ONCE, true>(p, rg, b, h, t0 + wave, t1, lane, qs, q, list, w_keys, w_scale, w_weights, st);
+  }
 
   // The waves' shares of each row, brought to the row's maximum and added.
   float* s_o = smem;                             // [4 waves][live][kMaskedRowPad]
   float* s_m = smem + 4 * live * kMaskedRowPad;  // [live][4 waves]
   float* s_l = s_m + 4 * live;
   __syncthreads();  // keys, scales and weights lay where the rows go
+  const float lsum = sum_xor<32>(sum_xor<16>(st.l[0]));
+  if (n < live) {
+    if (g == 0) s_m[4 * n + wave] = st.m[0], s_l[4 * n + wave] = lsum;
+    float* dst = s_o + (wave * live + n) * kMaskedRowPad + 32 * g;
 #pragma unroll
-  for (int r = 0; r < RT; ++r) {
-    const float l = sum_xor<32>(sum_xor<16>(st.l[r]));
-    const int row = 16 * r + n;
-    if (row < live) {
-      if (g == 0) s_m[4 * row + wave] = st.m[r], s_l[4 * row + wave] = l;
-      float* dst = s_o + (wave * live + row) * kMaskedRowPad + 32 * g;
+    for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int c = 0; c < 8; c += 4)
-          *(mf32x4*)(dst + 8 * i + c) = mf32x4{st.o[r][c][i], st.o[r][c + 1][i], st.o[r][c + 2][i], st.o[r][c + 3][i]};
-    }
+      for (int c = 0; c < 8; c += 4)
+        *(mf32x4*)(dst + 8 * i + c) = mf32x4{st.o[0][c][i], st.o[0][c + 1][i], st.o[0][c + 2][i], st.o[0][c + 3][i]};
   }
   __syncthreads();
-  const int64_t seg = (int64_t)b * p.Hkv + h, slot = seg * p.max_pieces + piece;
-  const float vscale = SK == kScaleHead ? p.vs[h] : 1.0f;
-#pragma unroll
-  for (int r = 0; r < RT; ++r) {
-    const int row = 16 * r + (tid >> 4), c = tid & 15;
-    if (row >= live) break;
+  const int64_t seg = ((int64_t)b * p.Hkv + h) * p.tiles + tile, slot = seg * p.max_pieces + piece;
+  const int row = tid >> 4, c = tid & 15;
+  if (row < live) {
     const mf32x4 m = *(const mf32x4*)(s_m + 4 * row), l = *(const mf32x4*)(s_l + 4 * row);
     const float M = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
     float L = 0.0f;
@@ -757,18 +805,18 @@ __global__ __launch_bounds__(256, RT == 1 ? 3 : 2) void masked_few_kernel(const 
       // Waves that saw nothing have no maximum, nor have those whose scores were all NaN, whose sums carry that on.
       const float a = m[w] == kNegInf ? (l[w] == 0.0f ? 0.0f : 1.0f) : fast_exp2(m[w] - M);
       const float* src = s_o + (w * live + row) * kMaskedRowPad + 2 * c;
-      if (a != 0.0f) L = fmaf(a, l[w], L);
+      L = fmaf(a, l[w], L);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const float2 x = *(const float2*)(src + 32 * i);
-        if (a != 0.0f) o.x[i][0] = fmaf(a, x.x, o.x[i][0]), o.x[i][1] = fmaf(a, x.y, o.x[i][1]);
+        o.x[i][0] = fmaf(a, x.x, o.x[i][0]), o.x[i][1] = fmaf(a, x.y, o.x[i][1]);
       }
     }
     const float inv = L == 0.0f ? 0.0f : vscale * __builtin_amdgcn_rcpf(L);
 #pragma unroll
     for (int i = 0; i < 4; ++i) o.x[i][0] *= inv, o.x[i][1] *= inv;
     const float lse2 = L == 0.0f ? kNegInf : (M == kNegInf ? 0.0f : M) + __log2f(L);
-    if (pieces == 1) masked_store_pairs(p, b, h, row, c, o, lse2);
+    if (pieces == 1) masked_store_pairs(p, b, h, r0 + row, c, o, lse2);
     else masked_store_partial(p, slot, row, c, o, lse2);
   }
   if (pieces == 1) return;
@@ -777,7 +825,7 @@ __global__ __launch_bounds__(256, RT == 1 ? 3 : 2) void masked_few_kernel(const 
   if (tid == 0) s_last = ws_arrive(p.counters + seg) == (unsigned)pieces - 1u;
   __syncthreads();
   if (!s_last) return;
-  masked_combine<256>(p, b, h, 0, live, seg * p.max_pieces, pieces, tid);
+  masked_combine<256>(p, b, h, r0, live, seg * p.max_pieces, pieces, tid);
   if (tid == 0) __hip_atomic_store(p.counters + seg, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
@@ -802,13 +850,13 @@ __device__ __forceinline__ void masked_many_steps(const MaskedParams& p, const M
   int list = t0 < t1 ? masked_page_list<PU>(p, rg, b, t0 + my_step, 0, t1, lane) : 0;
   auto issue = [&](int t) {  // chunk at step t of the list; steps past the piece's last repeat it
     const int token0 = masked_token0(rg, min(t + my_step, t1 - 1));
-    const MaskedPages pages = masked_pages(list);
+    const MaskedSpot spot = masked_spot<PU>(p, h, masked_pages(list), token0, rg.len);
     list = masked_page_list<PU>(p, rg, b, t + 2 + my_step, 0, t1, lane);
     if (wave < 2) {
-      masked_issue_k<KV, PU, false>(p, b, h, token0, rg.len, pages, lane, raw);
-      if constexpr (SK == kScaleTokenHead) sc = masked_issue_scale<PU>(p, b, h, token0, rg.len, pages, lane);
+      masked_issue_k<KV, PU, false>(p, b, h, token0, rg.len, spot, lane, raw);
+      if constexpr (SK == kScaleTokenHead) sc = masked_issue_scale<PU>(p, b, h, token0, rg.len, spot, lane);
     } else {
-      masked_issue_v<KV, PU, false>(p, b, h, token0, rg.len, pages, lane, raw);
+      masked_issue_v<KV, PU, false>(p, b, h, token0, rg.len, spot, lane, raw);
     }
   };
   if (t0 < t1) issue(t0);
@@ -949,7 +997,7 @@ static hipError_t launch_masked_t(const MaskedParams& p, int rt, bool many, int 
   const int live = p.live_rows;
   // The merge's rows, or the operands, scales and weights that lie there before it.
   const size_t merge = (size_t)4 * live * (kMaskedRowPad + 2) * sizeof(float);
-  const size_t early = (size_t)(4 * 4 * kMaskedItem + 4 * 64 + 4 * kMaskedStep * 16) * sizeof(float);
+  const size_t early = (size_t)(16 * masked_key_units(KV) + 4 * 64 + 4 * kMaskedStep * 16) * sizeof(float);
   const size_t few = merge > early ? merge : early;
   hipError_t e = hipSuccess;
   auto run = [&](auto kernel, size_t lds) {
@@ -957,10 +1005,10 @@ static hipError_t launch_masked_t(const MaskedParams& p, int rt, bool many, int 
       e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
     if (e == hipSuccess) hipLaunchKernelGGL(kernel, dim3(grid), dim3(256), lds, stream, p);
   };
-  if (many && rt == 2) run(masked_many_kernel<KV, SK, PU, QS, 2>, kMaskedManyLds);
+  if (rt == 2) run(masked_many_kernel<KV, SK, PU, QS, 2>, kMaskedManyLds);
   else if (many) run(masked_many_kernel<KV, SK, PU, QS, 1>, kMaskedManyLds);
-  else if (rt == 2) run(masked_few_kernel<KV, SK, PU, QS, 2>, few);
-  else run(masked_few_kernel<KV, SK, PU, QS, 1>, few);
+  else if (p.tiles > 1) run(masked_few_kernel<KV, SK, PU, QS, false>, few);
+  else run(masked_few_kernel<KV, SK, PU, QS, true>, few);
   return e == hipSuccess ? hipGetLastError() : e;
 }
 

@@ -409,6 +409,7 @@ struct RotaryParams {
   int tokens_per_group;  // tokens of one workgroup
   int log_lanes;         // log2 of the lanes that hold a row
   int vec;               // rows can be loaded and stored 8 channels at a time
+  int vec_pool;          // pool rows can be stored 8 codes at a time
   float scaling, eps;
   const void* blocks;
   const void* offsets;

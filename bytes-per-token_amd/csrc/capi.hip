@@ -1234,9 +1234,10 @@ int rotary_params(const bpt_rotary_args* a, bool pool, bpt::RotaryParams* out, b
   const int half = a->rotary_dim / 2, elem = float_bytes(a->x_dtype);
   for (int i = 0; i < half; ++i) p.axis[i] = a->pair_axis[i];
   // A lane holds 8 pairs, or 16 of the channels behind them.
-  const int units = std::max((half + 7) / 8 + (a->head_dim - a->rotary_dim + 15) / 16, (a->head_dim + 15) / 16);
+  const int units = std::max((p.interleaved ? (a->rotary_dim + 15) / 16 : (half + 7) / 8) + (a->head_dim - a->rotary_dim + 15) / 16,
+                             (a->head_dim + 15) / 16);
   p.log_lanes = log2i(units);
-  p.vec = half % 8 == 0 && a->head_dim % 16 == 0 &&
+  p.vec = half % 8 == 0 && a->head_dim % 16 == 0 && (!a->q_norm || aligned16(a->q_norm)) && (!a->k_norm || aligned16(a->k_norm)) &&
           (!a->num_q_heads || (rows_aligned(a->q, a->q_stride_b, a->q_stride_q, a->q_stride_h, elem) &&
                                rows_aligned(a->q_out, a->q_out_stride_b, a->q_out_stride_q, a->q_out_stride_h, elem))) &&
           (!a->num_k_heads || (rows_aligned(a->k, a->k_stride_b, a->k_stride_q, a->k_stride_h, elem) &&
@@ -1244,7 +1245,9 @@ int rotary_params(const bpt_rotary_args* a, bool pool, bpt::RotaryParams* out, b
   const int rows = a->num_q_heads + (pool ? 2 : 1) * a->num_k_heads, at_once = 256 >> p.log_lanes;
   const int64_t fill = (at_once + rows - 1) / rows;  // tokens that give every thread a row
   const int64_t most = bpt::kRotaryMaxAngles / half;
-  p.tokens_per_group = (int)std::max<int64_t>(1, std::min(fill, most));
+  // Large calls take tokens enough for an angle a thread, which spreads the barrier and the float64 work over more rows.
+  const int64_t full = tokens >= 8 * bpt::kComputeUnits ? (256 + half - 1) / half : 1;
+  p.tokens_per_group = (int)std::max<int64_t>(1, std::min(std::max(fill, full), most));
   *out = p;
   return BPT_OK;
 }
@@ -1279,6 +1282,9 @@ int bpt_rotary_append(const bpt_rotary_args* a, const bpt_append_args* append, v
       append->new_stride_h != a->k_stride_h)
     return fail(BPT_ERR_INVALID_ARGUMENT, "%s: both halves must describe the same keys", fn);
   p.v = append->v;
+  const int64_t whole = append->kv_dtype == BPT_KV_BF16 ? 16 : 8;
+  p.vec_pool = ((uintptr_t)w.kc | (uintptr_t)w.vc) % whole == 0 && w.kv_sblk % whole == 0 && w.kv_stok % whole == 0 &&
+               w.kv_shead % whole == 0 && p.rot % 16 == 0;
   p.vec = p.vec && rows_aligned(append->v, p.k_sb, p.k_sq, p.k_sh, float_bytes(a->x_dtype));
   p.blocks = w.blocks;
   p.offsets = w.offsets;

@@ -95,14 +95,13 @@ def paged_masked_attention(
     if q.dtype == torch.float32:
         raise ValueError("q must be bf16 or f16")
     dev = q.device
-    if dev.type != "cuda":
+    if not q.is_cuda:
         raise ValueError("paged_masked_attention runs on a GPU: q must be a cuda tensor")
-    for name, t in (("k_cache", k_cache), ("v_cache", v_cache), ("block_table", block_table), ("context_lens", context_lens),
-                    ("k_scale", k_scale), ("v_scale", v_scale), ("slopes", slopes), ("prefix_lens", prefix_lens), ("starts", starts)):
+    for t in (k_cache, v_cache, block_table, context_lens, k_scale, v_scale, slopes, prefix_lens, starts):
         if t is not None and t.device != dev:
-            raise ValueError(f"{name} is on {t.device}, q on {dev}")
+            raise ValueError(f"a tensor of the call is on {t.device}, q on {dev}")
     if out is None:
-        out4 = torch.empty((b, nq, hq, d), dtype=out_dtype, device=dev)
+        out4 = q.new_empty((b, nq, hq, d), dtype=out_dtype)
     else:
         out4 = out[:, None] if out.dim() == 3 else out
         if tuple(out4.shape) != (b, nq, hq, d):
@@ -121,7 +120,7 @@ def paged_masked_attention(
         if workspace is None or counters is None:
             ws_bytes, cnt_bytes = ctypes.c_size_t(), ctypes.c_size_t()
             _lib.check(lib.bpt_masked_plan(a, m, ws_bytes, cnt_bytes))
-            if torch.cuda.is_current_stream_capturing():
+            if torch._C._cuda_isCurrentStreamCapturing():
                 # Captures share one stream, but their graphs may be replayed at once: each call gets buffers of its own, from
                 # its graph's pool, and the counters' clearing is part of the graph.
                 workspace = torch.empty(ws_bytes.value, dtype=torch.uint8, device=dev) if workspace is None else workspace

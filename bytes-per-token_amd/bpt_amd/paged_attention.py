@@ -63,7 +63,7 @@ _HERE = contextlib.nullcontext()
 
 def _on_device(device: torch.device):
     """Makes `device` the current one where it is not: kernels are launched on the current device."""
-    return _HERE if device.index is None or device.index == torch.cuda.current_device() else torch.cuda.device(device)
+    return _HERE if device.index is None or device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)
 
 
 def _scale_layout(k_scale, v_scale, kv_code: int, pool_shape) -> tuple[int, tuple[int, int, int]]:

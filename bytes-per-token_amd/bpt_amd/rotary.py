@@ -59,7 +59,7 @@ def _check_rows(name: str, x: torch.Tensor, like: torch.Tensor | None = None) ->
 
 def _out_like(name: str, out: torch.Tensor | None, x: torch.Tensor) -> torch.Tensor:
     if out is None:
-        return torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        return x.new_empty(x.shape)
     if out.shape != x.shape or out.dtype != x.dtype or out.device != x.device or out.stride(-1) != 1:
         raise ValueError(f"{name} must be {tuple(x.shape)} in {x.dtype} on {x.device}, channels contiguous")
     if any(n > 1 and s == 0 for n, s in zip(out.shape, out.stride())):
@@ -70,7 +70,8 @@ def _out_like(name: str, out: torch.Tensor | None, x: torch.Tensor) -> torch.Ten
 def _rotary_args(q, k, q_out, k_out, positions, inv_freq, sections, cyclic, interleaved, scaling, q_norm, k_norm, eps):
     """The checked bpt_rotary_args."""
     b, n, hq, d = q.shape
-    if positions.dim() not in (2, 3) or tuple(positions.shape[-2:]) != (b, n) or positions.dtype not in _INDEX_CODES:
+    pos_shape, pos_code = positions.shape, _INDEX_CODES.get(positions.dtype)
+    if len(pos_shape) not in (2, 3) or pos_shape[-2:] != (b, n) or pos_code is None:
         raise ValueError(f"positions must be int32 / int64 [{b}, {n}] or [axes, {b}, {n}], got {tuple(positions.shape)}")
     if inv_freq.dim() != 1 or inv_freq.dtype != torch.float32 or not inv_freq.is_contiguous():
         raise ValueError("inv_freq must be a contiguous float32 [rotary_dim / 2]")
@@ -78,29 +79,36 @@ def _rotary_args(q, k, q_out, k_out, positions, inv_freq, sections, cyclic, inte
     if not 1 <= half <= d // 2 or d % 2 or d > 256:
         raise ValueError(f"{half} pairs do not fit into head_dim {d} (even, at most 256)")
     norm_code = 0
-    for name, w in (("q_norm", q_norm), ("k_norm", k_norm)):
+    for w in (q_norm, k_norm):
         if w is not None:
-            if tuple(w.shape) != (d,) or w.dtype not in _FLOAT_CODES or not w.is_contiguous():
-                raise ValueError(f"{name} must be a contiguous bf16 / f16 / f32 [{d}]")
+            if w.shape != (d,) or w.dtype not in _FLOAT_CODES or not w.is_contiguous():
+                raise ValueError(f"q_norm and k_norm must be contiguous bf16 / f16 / f32 [{d}]")
             norm_code = _FLOAT_CODES[w.dtype]
     if q_norm is not None and k_norm is not None and q_norm.dtype != k_norm.dtype:
         raise ValueError("q_norm and k_norm must share a dtype")
     dev = q.device
-    if dev.type != "cuda":
+    if not q.is_cuda:
         raise ValueError("rotary positions are applied on a GPU: q must be a cuda tensor")
-    for name, t in (("positions", positions), ("inv_freq", inv_freq), ("q_norm", q_norm), ("k_norm", k_norm)):
-        if t is not None and t.device != dev:
-            raise ValueError(f"{name} is on {t.device}, q on {dev}")
-    axes = 1 if positions.dim() == 2 else positions.shape[0]
+    if positions.device != dev or inv_freq.device != dev or (q_norm is not None and q_norm.device != dev) or (
+            k_norm is not None and k_norm.device != dev):
+        raise ValueError(f"positions, inv_freq and norm weights must be on q's device {dev}")
+    axes = 1 if len(pos_shape) == 2 else pos_shape[0]
     which = pair_axes(half, axes, None if sections is None else tuple(sections), bool(cyclic))
-    pos_sa, pos_sb, pos_sq = (0, *positions.stride()) if positions.dim() == 2 else positions.stride()
-    k_rows = (None, 0, 0, 0) if k is None else (k.data_ptr(), *k.stride()[:3])
-    ko_rows = (None, 0, 0, 0) if k_out is None else (k_out.data_ptr(), *k_out.stride()[:3])
+    pos_sa, pos_sb, pos_sq = (0, *positions.stride()) if len(pos_shape) == 2 else positions.stride()
+    q_sb, q_sq, q_sh, _ = q.stride()
+    qo_sb, qo_sq, qo_sh, _ = q_out.stride()
+    k_ptr = ko_ptr = None
+    k_sb = k_sq = k_sh = ko_sb = ko_sq = ko_sh = hk = 0
+    if k is not None:
+        k_ptr, hk = k.data_ptr(), k.shape[2]
+        k_sb, k_sq, k_sh, _ = k.stride()
+    if k_out is not None:
+        ko_ptr = k_out.data_ptr()
+        ko_sb, ko_sq, ko_sh, _ = k_out.stride()
     # The fields of bpt_rotary_args in order, up to pair_axis.
     a = _lib.RotaryArgs(
-        _lib.ROTARY_ARGS_SIZE, _FLOAT_CODES[q.dtype], norm_code, _INDEX_CODES[positions.dtype], b, n, hq,
-        0 if k is None else k.shape[2], d, 2 * half, axes, bool(interleaved), float(scaling), float(eps), q.data_ptr(),
-        *q.stride()[:3], *k_rows, q_out.data_ptr(), *q_out.stride()[:3], *ko_rows,
+        _lib.ROTARY_ARGS_SIZE, _FLOAT_CODES[q.dtype], norm_code, pos_code, b, n, hq, hk, d, 2 * half, axes, bool(interleaved), scaling,
+        eps, q.data_ptr(), q_sb, q_sq, q_sh, k_ptr, k_sb, k_sq, k_sh, q_out.data_ptr(), qo_sb, qo_sq, qo_sh, ko_ptr, ko_sb, ko_sq, ko_sh,
         None if q_norm is None else q_norm.data_ptr(), None if k_norm is None else k_norm.data_ptr(), inv_freq.data_ptr(),
         positions.data_ptr(), pos_sa, pos_sb, pos_sq,
     )

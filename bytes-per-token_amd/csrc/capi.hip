@@ -1245,8 +1245,9 @@ int rotary_params(const bpt_rotary_args* a, bool pool, bpt::RotaryParams* out, b
   const int rows = a->num_q_heads + (pool ? 2 : 1) * a->num_k_heads, at_once = 256 >> p.log_lanes;
   const int64_t fill = (at_once + rows - 1) / rows;  // tokens that give every thread a row
   const int64_t most = bpt::kRotaryMaxAngles / half;
-  // Large calls take tokens enough for an angle a thread, which spreads the barrier and the float64 work over more rows.
-  const int64_t full = tokens >= 8 * bpt::kComputeUnits ? (256 + half - 1) / half : 1;
+  // Large calls take two tokens at least, which spreads the barrier and the float64 work over more rows; more of them leave a
+  // longer tail. FP8 append of 4 x 4096 tokens (32 + 8 heads), 1 / 2 / 3 / 4 tokens: 117 / 98 / 103 / 99 us, INT8 of 2048: - / 60 / 66 / 68.
+  const int64_t full = tokens >= 8 * bpt::kComputeUnits ? 2 : 1;
   p.tokens_per_group = (int)std::max<int64_t>(1, std::min(std::max(fill, full), most));
   *out = p;
   return BPT_OK;

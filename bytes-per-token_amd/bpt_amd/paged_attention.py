@@ -94,49 +94,55 @@ def _scale_layout(k_scale, v_scale, kv_code: int, pool_shape) -> tuple[int, tupl
 def _decode_args(
     q, k_cache, v_cache, block_table, context_lens, k_scale, v_scale, scale, max_context, num_splits, out_dtype
 ) -> tuple[_lib.DecodeArgs, tuple[int, int, int, int]]:
-    if q.dim() != 4:
-        raise ValueError(f"q must be [B, Q, Hq, D], got {tuple(q.shape)}")
-    b, nq, hq, d = q.shape
-    if q.dtype not in _FLOAT_CODES:
+    shape, strides = q.shape, q.stride()
+    if len(shape) != 4:
+        raise ValueError(f"q must be [B, Q, Hq, D], got {tuple(shape)}")
+    b, nq, hq, d = shape
+    q_code = _FLOAT_CODES.get(q.dtype)
+    if q_code is None:
         raise ValueError(f"q must be bf16, f16 or f32, got {q.dtype}")
-    if q.stride(-1) != 1:
+    q_sb, q_sq, q_sh, q_sd = strides
+    if q_sd != 1:
         raise ValueError("q's channel dimension must be contiguous")
-    if not (k_cache.dim() == 4 and k_cache.shape == v_cache.shape):
+    pool, kv_dtype, kv_strides = k_cache.shape, k_cache.dtype, k_cache.stride()
+    if not (len(pool) == 4 and pool == v_cache.shape):
         raise ValueError("k_cache and v_cache must be [NB, P, Hkv, D]")
-    if k_cache.dtype != v_cache.dtype:
+    if kv_dtype != v_cache.dtype:
         raise ValueError("k_cache and v_cache must share a dtype")
-    if k_cache.stride() != v_cache.stride():
+    if kv_strides != v_cache.stride():
         raise ValueError("k_cache and v_cache must share strides")
-    if k_cache.stride(-1) != 1:
+    kv_sb, kv_st, kv_sh, kv_sd = kv_strides
+    if kv_sd != 1:
         raise ValueError("the caches' channel dimension must be contiguous")
-    kv_code = kv_dtype_code(k_cache.dtype)
-    nb, page, hkv, dk = k_cache.shape
+    kv_code = kv_dtype_code(kv_dtype)
+    nb, page, hkv, dk = pool
     if dk != d:
         raise ValueError(f"q head_dim {d} != cache head_dim {dk}")
-    if not (block_table.dim() == 2 and block_table.shape[0] == b):
+    table_shape = block_table.shape
+    if not (len(table_shape) == 2 and table_shape[0] == b):
         raise ValueError(f"block_table must be [{b}, max_blocks]")
-    if block_table.dtype not in _INDEX_CODES:
+    table_code = _INDEX_CODES.get(block_table.dtype)
+    if table_code is None:
         raise ValueError("block_table must be int32 or int64")
-    if block_table.stride(1) != 1:
+    table_sb, table_s1 = block_table.stride()
+    if table_s1 != 1:
         raise ValueError("block_table rows must be contiguous")
     if context_lens is not None:
         if not (context_lens.dim() == 1 and context_lens.shape[0] == b):
             raise ValueError(f"context_lens must be [{b}]")
         if not (context_lens.dtype == torch.int32 and context_lens.is_contiguous()):
             raise ValueError("context_lens must be contiguous int32")
-    if out_dtype not in _FLOAT_CODES:
+    out_code = _FLOAT_CODES.get(out_dtype)
+    if out_code is None:
         raise ValueError(f"out dtype must be bf16, f16 or f32, got {out_dtype}")
-    scale_kind, sc_strides = _scale_layout(k_scale, v_scale, kv_code, k_cache.shape)
+    scale_kind, sc_strides = _scale_layout(k_scale, v_scale, kv_code, pool)
 
-    q_sb, q_sq, q_sh, _ = q.stride()
-    kv_sb, kv_st, kv_sh, _ = k_cache.stride()
     # The fields of bpt_decode_args in order, up to context_lens (one call: a field at a time costs twice as much).
     a = _lib.DecodeArgs(
-        _lib.DECODE_ARGS_SIZE, kv_code, scale_kind, _FLOAT_CODES[q.dtype], _FLOAT_CODES[out_dtype],
-        _INDEX_CODES[block_table.dtype], b, nq, hq, hkv, d, page, nb, block_table.shape[1], int(max_context),
-        int(num_splits or 0), 0, 0, 0, float(scale), q.data_ptr(), q_sb, q_sq, q_sh, k_cache.data_ptr(),
+        _lib.DECODE_ARGS_SIZE, kv_code, scale_kind, q_code, out_code, table_code, b, nq, hq, hkv, d, page, nb, table_shape[1],
+        int(max_context), int(num_splits or 0), 0, 0, 0, float(scale), q.data_ptr(), q_sb, q_sq, q_sh, k_cache.data_ptr(),
         v_cache.data_ptr(), kv_sb, kv_st, kv_sh, None if k_scale is None else k_scale.data_ptr(),
-        None if v_scale is None else v_scale.data_ptr(), *sc_strides, block_table.data_ptr(), block_table.stride(0),
+        None if v_scale is None else v_scale.data_ptr(), *sc_strides, block_table.data_ptr(), table_sb,
         None if context_lens is None else context_lens.data_ptr(),
     )
     return a, (b, nq, hq, d)
@@ -324,45 +330,52 @@ def quantize_append(
 
 def _append_args(k, v, k_cache, v_cache, k_scale, v_scale, write_blocks, write_offsets):
     """The checked bpt_append_args of quantize_append's arguments, and their device."""
-    if not (k.dim() == 4 and k.shape == v.shape):
+    shape, dtype, strides = k.shape, k.dtype, k.stride()
+    src_code = _FLOAT_CODES.get(dtype)
+    if not (len(shape) == 4 and shape == v.shape):
         raise ValueError("k and v must be [B, Q, Hkv, D]")
-    if not (k.dtype == v.dtype and k.dtype in _FLOAT_CODES):
+    if not (dtype == v.dtype and src_code is not None):
         raise ValueError("k and v must share a bf16/f16/f32 dtype")
-    if not (k.stride() == v.stride() and k.stride(-1) == 1):
+    n_sb, n_sq, n_sh, n_sd = strides
+    if not (strides == v.stride() and n_sd == 1):
         raise ValueError("k and v must share strides, channels contiguous")
-    b, nq, hkv, d = k.shape
-    if not (k_cache.dim() == 4 and k_cache.shape == v_cache.shape):
+    b, nq, hkv, d = shape
+    pool, kv_dtype, kv_strides = k_cache.shape, k_cache.dtype, k_cache.stride()
+    if not (len(pool) == 4 and pool == v_cache.shape):
         raise ValueError("k_cache and v_cache must be [NB, P, Hkv, D]")
-    if not (k_cache.dtype == v_cache.dtype and k_cache.stride() == v_cache.stride()):
+    if not (kv_dtype == v_cache.dtype and kv_strides == v_cache.stride()):
         raise ValueError("caches must match")
-    if not (k_cache.shape[2] == hkv and k_cache.shape[3] == d):
+    nb, page, pool_heads, pool_d = pool
+    if not (pool_heads == hkv and pool_d == d):
         raise ValueError("cache heads/head_dim must match the rows")
-    if k_cache.stride(-1) != 1:
+    kv_sb, kv_st, kv_sh, kv_sd = kv_strides
+    if kv_sd != 1:
         raise ValueError("the caches' channel dimension must be contiguous")
-    kv_code = kv_dtype_code(k_cache.dtype)
-    scale_kind, sc_strides = _scale_layout(k_scale, v_scale, kv_code, k_cache.shape)
+    kv_code = kv_dtype_code(kv_dtype)
+    scale_kind, sc_strides = _scale_layout(k_scale, v_scale, kv_code, pool)
     if not (write_blocks.shape == (b, nq) and write_offsets.shape == (b, nq)):
         raise ValueError(f"write slots must be [{b}, {nq}]")
-    if not (write_blocks.dtype == write_offsets.dtype and write_blocks.dtype in _INDEX_CODES):
+    slot_code = _INDEX_CODES.get(write_blocks.dtype)
+    if not (write_blocks.dtype == write_offsets.dtype and slot_code is not None):
         raise ValueError("slots: int32/int64")
-    if write_blocks.stride() != write_offsets.stride():
+    slot_strides = write_blocks.stride()
+    if slot_strides != write_offsets.stride():
         raise ValueError("write_blocks and write_offsets must share strides")
     dev = k.device
-    if dev.type != "cuda":
+    if not k.is_cuda:
         raise ValueError("quantize_append runs on a GPU: k must be a cuda tensor")
-    for name, t in (("v", v), ("k_cache", k_cache), ("v_cache", v_cache), ("write_blocks", write_blocks),
-                    ("write_offsets", write_offsets), ("k_scale", k_scale), ("v_scale", v_scale)):
+    for t in (v, k_cache, v_cache, write_blocks, write_offsets, k_scale, v_scale):
         if t is not None and t.device != dev:
-            raise ValueError(f"{name} is not on {dev}")
+            for name, t in (("v", v), ("k_cache", k_cache), ("v_cache", v_cache), ("write_blocks", write_blocks),
+                            ("write_offsets", write_offsets), ("k_scale", k_scale), ("v_scale", v_scale)):
+                if t is not None and t.device != dev:
+                    raise ValueError(f"{name} is not on {dev}")
 
-    n_sb, n_sq, n_sh, _ = k.stride()
-    kv_sb, kv_st, kv_sh, _ = k_cache.stride()
     # The fields of bpt_append_args in order.
     a = _lib.AppendArgs(
-        _lib.APPEND_ARGS_SIZE, kv_code, scale_kind, _FLOAT_CODES[k.dtype], _INDEX_CODES[write_blocks.dtype], b, nq, hkv,
-        d, k_cache.shape[1], k_cache.shape[0], k.data_ptr(), v.data_ptr(), n_sb, n_sq, n_sh, write_blocks.data_ptr(),
-        write_offsets.data_ptr(), *write_blocks.stride(), k_cache.data_ptr(), v_cache.data_ptr(), kv_sb, kv_st, kv_sh,
-        None if k_scale is None else k_scale.data_ptr(), None if v_scale is None else v_scale.data_ptr(), *sc_strides,
+        _lib.APPEND_ARGS_SIZE, kv_code, scale_kind, src_code, slot_code, b, nq, hkv, d, page, nb, k.data_ptr(), v.data_ptr(), n_sb,
+        n_sq, n_sh, write_blocks.data_ptr(), write_offsets.data_ptr(), *slot_strides, k_cache.data_ptr(), v_cache.data_ptr(), kv_sb,
+        kv_st, kv_sh, None if k_scale is None else k_scale.data_ptr(), None if v_scale is None else v_scale.data_ptr(), *sc_strides,
     )
     return a, dev
 

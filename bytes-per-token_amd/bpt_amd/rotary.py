@@ -46,7 +46,7 @@ def pair_axes(half: int, axes: int, sections: tuple[int, ...] | None, cyclic: bo
 
 
 def _check_rows(name: str, x: torch.Tensor, like: torch.Tensor | None = None) -> None:
-    if x.dim() != 4 or x.stride(-1) != 1:
+    if x.dim() != 4 or x.stride(3) != 1:
         raise ValueError(f"{name} must be [B, Q, H, D] with contiguous channels, got {tuple(x.shape)}")
     if x.dtype not in _FLOAT_CODES:
         raise ValueError(f"{name} must be bf16, f16 or f32, got {x.dtype}")
@@ -185,8 +185,9 @@ def rotary_append(
     slots as quantize_append's, head_dim 64, 128 or 256; the other arguments as rotary_embed's.
     """
     _check_rows("q", q)
-    _check_rows("k", k, q)
-    w, _ = _append_args(k, v, k_cache, v_cache, k_scale, v_scale, write_blocks, write_offsets)
+    w, dev = _append_args(k, v, k_cache, v_cache, k_scale, v_scale, write_blocks, write_offsets)
+    if k.dtype != q.dtype or q.device != dev or q.shape[:2] != k.shape[:2] or q.shape[3] != k.shape[3]:
+        raise ValueError(f"q must have k's dtype, device, batch, queries and head_dim, got {q.dtype} {tuple(q.shape)}, k {tuple(k.shape)}")
     q_out = _out_like("q_out", q_out, q)
     a = _rotary_args(q, k, q_out, None, positions, inv_freq, sections, cyclic, interleaved, scaling, q_norm, k_norm, eps)
     with _on_device(q.device):

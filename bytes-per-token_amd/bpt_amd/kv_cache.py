@@ -16,7 +16,9 @@ The drop-in for fastserve's engine (paths relative to its src/fastserve/):
   one (engine/model.py:72-74, contract of integration/kv_cache.py:160-168): the step's keys and values are
   quantized into their slots first (store before attend), then one fused paged decode attention reads the
   codes; a query at position p sees the slots 0..p of its row (engine/attention.py:12-20), so decode steps
-  (Q = 1), speculative verify steps (Q = k + 1) and prefill chunks all go through the same kernel.
+  (Q = 1), speculative verify steps (Q = k + 1) and prefill chunks all go through the same kernel. With `rotary` the keys and
+  queries are normalised and rotated on the way (rotary.py), with `mask` scores are capped, biased and masked beyond the
+  causal rule (masked_attention.py).
 * `update` raises, as QuantizedKVCache.update does (integration/kv_cache.py:136-137): the cache never hands
   out float keys and values.
 
@@ -32,7 +34,9 @@ from typing import Any
 
 import torch
 
-from .paged_attention import paged_append_decode, paged_prepare
+from . import _lib, masked_attention
+from .paged_attention import decode_plan, paged_append_decode, paged_decode_attention, paged_prepare, quantize_append
+from .rotary import rotary_append
 
 _FORMATS = {torch.float8_e4m3fn: "fp8", torch.int8: "int8", torch.bfloat16: "bf16"}
 HEAD_DIM = 128  # the one head size the paged decode kernels are built for
@@ -238,18 +242,43 @@ class PagedQuantKVCache:
         raise NotImplementedError("a quantized cache never returns float keys and values: use attend()")
 
     def attend(
-        self, layer: int, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, meta: PagedMeta, scale: float
+        self, layer: int, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, meta: PagedMeta, scale: float, *,
+        rotary: dict | None = None, mask: dict | None = None,
     ) -> torch.Tensor:
-        """Store this step's k, v [B, Hkv, Q, D] in their slots, then attend: q [B, Hq, Q, D] -> [B, Hq, Q, D]."""
+        """Store this step's k, v [B, Hkv, Q, D] in their slots, then attend: q [B, Hq, Q, D] -> [B, Hq, Q, D].
+
+        rotary  for q and k as the projections leave them: rotary_append's arguments (positions [B, Q] or [axes, B, Q] and
+                inv_freq, and as needed sections, cyclic, interleaved, scaling, q_norm, k_norm, eps). The keys are then rotated on
+                their way into the cache.
+        mask    paged_masked_attention's arguments beyond the causal mask: softcap, slopes, window, prefix_lens, max_prefix,
+                starts.
+        """
         b, hq, nq, d = q.shape
         if tuple(k.shape) != (b, self.num_kv_heads, nq, d) or k.shape != v.shape:
             raise ValueError(f"k and v must be [{b}, {self.num_kv_heads}, {nq}, {d}]")
         if tuple(meta.write_blocks.shape) != (b, nq):
             raise ValueError(f"meta was prepared for {tuple(meta.write_blocks.shape)} tokens, not {(b, nq)}")
-        # Store, then attend; one launch where the decode kernel can store the rows itself (paged_append_decode).
-        out = paged_append_decode(
-            q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2), self.k[layer], self.v[layer], meta.block_table,
-            meta.context_lens, self.k_scale[layer], self.v_scale[layer], meta.write_blocks, meta.write_offsets,
-            scale=scale, max_context=meta.kv_len, out_dtype=q.dtype,
-        )  # [B, Q, Hq, D] in q's dtype: the kernel rounds once, from float32 (integration/kv_cache.py:177-181)
+        pools = (self.k[layer], self.v[layer])
+        scales = (self.k_scale[layer], self.v_scale[layer])
+        slots = (meta.write_blocks, meta.write_offsets)
+        q, k, v = q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2)
+        how = dict(scale=scale, max_context=meta.kv_len, out_dtype=q.dtype)
+        if not rotary and not mask:
+            # Store, then attend; one launch where the decode kernel can store the rows itself (paged_append_decode).
+            out = paged_append_decode(q, k, v, *pools, meta.block_table, meta.context_lens, *scales, *slots, **how)
+            return out.transpose(1, 2)  # [B, Q, Hq, D] in q's dtype: the kernel rounds once, from float32 (integration/kv_cache.py:177-181)
+        # Both halves' arguments are checked before anything is stored.
+        turned = q.new_empty(q.shape) if rotary else q
+        args = (turned, *pools, meta.block_table, meta.context_lens, *scales)
+        if mask:
+            call = masked_attention._checked(*args, **mask, **how)
+            _lib.check(_lib.lib().bpt_masked_plan(call[0], call[1], None, None))
+        else:
+            decode_plan(*args, scale=scale, max_context=meta.kv_len)
+        if rotary:
+            rest = {name: x for name, x in rotary.items() if name not in ("positions", "inv_freq")}
+            rotary_append(q, k, v, rotary["positions"], rotary["inv_freq"], *pools, *scales, *slots, q_out=turned, **rest)
+        else:
+            quantize_append(k, v, *pools, *scales, *slots)
+        out = masked_attention._launch(*call) if mask else paged_decode_attention(*args, **how)
         return out.transpose(1, 2)

@@ -87,8 +87,16 @@ def paged_masked_attention(
 
     Returns [B, Q, Hq, D] (or [B, Hq, D] for a 3-D q with one query per sequence) in out_dtype.
     """
-    squeeze = q.dim() == 3
-    q4 = q[:, None] if squeeze else q
+    call = _checked(q, k_cache, v_cache, block_table, context_lens, k_scale, v_scale, scale, max_context, softcap, slopes, window,
+                    prefix_lens, max_prefix, starts, out, out_dtype, lse)
+    result = _launch(*call, workspace, counters)
+    return result[:, 0] if (q.dim() == 3 and result.dim() == 4) else result
+
+
+def _checked(q, k_cache, v_cache, block_table, context_lens, k_scale, v_scale, scale, max_context, softcap=None, slopes=None, window=None,
+             prefix_lens=None, max_prefix=None, starts=None, out=None, out_dtype=torch.bfloat16, lse=None):
+    """Everything of a call that can be refused, apart from its buffers: (decode args, mask args, device, result)."""
+    q4 = q[:, None] if q.dim() == 3 else q
     a, (b, nq, hq, d) = _decode_args(q4, k_cache, v_cache, block_table, context_lens, k_scale, v_scale, scale, max_context, None,
                                      out.dtype if out is not None else out_dtype)
     m = _mask_args(b, nq, hq, int(max_context), softcap, slopes, window, prefix_lens, max_prefix, starts)
@@ -114,6 +122,10 @@ def paged_masked_attention(
         if not (lse.dtype == torch.float32 and lse.is_contiguous() and lse.numel() == b * nq * hq and lse.device == dev):
             raise ValueError(f"lse must be a contiguous float32 tensor of {b} x {nq} x {hq} on q's device")
         a.lse_out = lse.data_ptr()
+    return a, m, dev, out if out is not None else out4
+
+
+def _launch(a, m, dev, result, workspace=None, counters=None) -> torch.Tensor:
     lib = _lib.lib()
     with _on_device(dev):
         stream = _stream(dev)
@@ -134,8 +146,7 @@ def paged_masked_attention(
         a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.nbytes
         a.counters, a.counters_bytes = counters.data_ptr(), counters.nbytes
         _lib.check(lib.bpt_paged_masked(a, m, stream))
-    result = out if out is not None else out4
-    return result[:, 0] if (squeeze and result.dim() == 4) else result
+    return result
 
 
 def masked_plan(q, k_cache, v_cache, block_table, context_lens, k_scale=None, v_scale=None, *, scale, max_context, softcap=None,

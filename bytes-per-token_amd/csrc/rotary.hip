@@ -97,7 +97,7 @@ __device__ __forceinline__ void rotary_load_weights(const void* w, int c, int dt
 
 // x / s to where it rounds to the same e4m3 code, given inv = 1 / s to an ulp: the product is within 2^-22 of the quotient, and
 // midpoints of normal codes (magnitudes from 2^-6 on) have nothing below the mantissa's bit 19. Products within 4 ulps of one, and
-// those below the normal range, take the IEEE division; so do NaN and scales whose reciprocal is not a normal number.
+// those below the normal range, take the IEEE division, as do NaN and (rotary_store_codes) scales past 2^+-100.
 __device__ __forceinline__ bool rotary_fp8_sure(float q) {
   const uint32_t u = __float_as_uint(q);
   return (u & 0x7fffffffu) >= 0x3c800000u && (u & 0x7fffffffu) < 0x7f000000u && ((u & 0xfffffu) - 0x7fffcu) > 8u;
@@ -116,9 +116,10 @@ __device__ __forceinline__ void rotary_store_codes(uint8_t* dst, const float* x,
     }
   } else {
     uint32_t code[8];
+    const bool normal = s >= 0x1p-100f && s <= 0x1p100f;  // far enough inside that the reciprocal is a normal number too
     if constexpr (KV == kKvFp8) {
       float y[8];
-      bool sure = true;
+      bool sure = normal;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         y[j] = x[j] * inv;
@@ -133,7 +134,7 @@ __device__ __forceinline__ void rotary_store_codes(uint8_t* dst, const float* x,
     } else {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        float r = s >= 0x1p-100f ? rint_quotient(x[j], s, inv) : rintf(__fdiv_rn(x[j], s));
+        float r = normal ? rint_quotient(x[j], s, inv) : rintf(__fdiv_rn(x[j], s));
         r = r > 127.0f ? 127.0f : (r < -128.0f ? -128.0f : r);
         code[j] = (uint32_t)(int32_t)r & 0xffu;
       }

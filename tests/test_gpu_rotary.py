@@ -215,6 +215,71 @@ def test_append_matches_quantize_append_on_unrotated_rows():
             assert (x is None and y is None) or torch.equal(x.contiguous().view(torch.uint8), y.contiguous().view(torch.uint8))
 
 
+SCALES = [1.0, 0.0137, 3e-5, 7.7, 2.0**-10, 1e-12, 2.0**101, 2.0**127, 3e38, 2.0**-101, 1e-39, 0.0, -0.25, float("inf"), float("nan")]
+
+
+def stored_alike(fmt, per_token, x, scales):
+    """rotary_append stores the values x [N, D] under every scale as quantize_append does, bit for bit (any NaN as any other)."""
+    from bpt_amd import quantize_append, rotary_append
+
+    heads = 1 if per_token else len(scales)
+    n, d = x.shape
+    v = x[None, :, None].expand(1, n, heads, d).contiguous()
+    q, nb = torch.zeros_like(v), -(-n // 16)
+    at = torch.arange(n, device=DEV, dtype=torch.int32)[None]
+    got, want = [], []
+    for out in (got, want):
+        k_cache, v_cache, ks, vs = pools(fmt, nb, 16, heads, d, per_token)
+        if fmt != "bf16" and not per_token:
+            ks, vs = torch.ones(heads, device=DEV), torch.tensor(scales, device=DEV)
+        if out is got:
+            rotary_append(q, torch.zeros_like(v), v, at, freqs(d // 2), k_cache, v_cache, ks, vs, at // 16, at % 16)
+        else:
+            quantize_append(torch.zeros_like(v), v, k_cache, v_cache, ks, vs, at // 16, at % 16)
+        torch.cuda.synchronize()
+        out += [v_cache.float(), v_cache.view(torch.uint8)] + ([vs] if per_token else [])
+    if per_token:
+        # The maximum of a row with a signalling NaN depends on the order it is taken in: max(x, sNaN) is a NaN, which max(NaN, y)
+        # then drops. Such rows are left out.
+        bits, top = (x.view(torch.int16).int() & 0x7FFF), {torch.bfloat16: (0x7F80, 0x40), torch.float16: (0x7C00, 0x200)}[x.dtype]
+        keep = torch.ones(nb * 16, dtype=torch.bool, device=DEV)
+        keep[:n] = ~((bits > top[0]) & (bits & top[1] == 0)).any(-1)
+        for out in (got, want):
+            out[:] = [t.flatten(0, 1)[keep] for t in out]
+    nan = torch.isnan(got[0])
+    assert torch.equal(nan, torch.isnan(want[0]))
+    each = nan.repeat_interleave(got[1].shape[-1] // d, -1)
+    bad = (got[1] != want[1]) & ~each
+    assert not bad.any(), f"{int(bad.sum())} codes differ, first at {bad.nonzero()[0].tolist()}"
+    assert all(torch.equal(a, b) for a, b in zip(got[2:], want[2:]))
+
+
+@pytest.mark.parametrize("fmt, per_token", [("bf16", False), ("fp8", False), ("fp8", True), ("int8", False), ("int8", True)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_every_16_bit_value_is_stored_as_quantize_append_stores_it(fmt, per_token, dtype):
+    bits = torch.arange(65536, dtype=torch.int32, device=DEV).to(torch.int16).view(dtype)
+    stored_alike(fmt, per_token, bits.reshape(512, 128), SCALES)
+    stored_alike(fmt, per_token, bits.reshape(128, 512).T.reshape(512, 128), SCALES)  # magnitudes far apart in a row
+
+
+@pytest.mark.parametrize("fmt", ["fp8", "int8"])
+def test_values_next_to_the_midpoints_of_codes(fmt):
+    """Where a product with the scale's reciprocal and the division could round apart."""
+    if fmt == "fp8":
+        codes = torch.arange(127, dtype=torch.uint8, device=DEV).view(torch.float8_e4m3fn).double()
+        mid = (codes[1:] + codes[:-1]) / 2
+    else:
+        mid = torch.arange(127, device=DEV).double() + 0.5
+    scales = [s for s in SCALES if 0 < s < 2.0**100] + [0.3 + 0.0007 * i for i in range(24)]
+    for s in scales:
+        near = (mid * float(np.float32(s))).float()
+        up = torch.nextafter(near, torch.full_like(near, float("inf")))
+        down = torch.nextafter(near, torch.zeros_like(near))
+        x = torch.cat([near, up, down, -near, -up, -down, torch.zeros(24 if len(mid) == 126 else 6, device=DEV)])
+        x = torch.cat([x, torch.zeros(-len(x) % 128, device=DEV)]).reshape(-1, 128)
+        stored_alike(fmt, False, x, [s])
+
+
 def test_nan_and_infinity_stay_in_their_pair():
     from bpt_amd import rotary_embed
 

@@ -22,8 +22,8 @@ from .paged_attention import _decode_args, _on_device, _stream, cached_buffer
 
 def _mask_args(b, nq, hq, max_context, softcap, slopes, window, prefix_lens, max_prefix, starts) -> _lib.MaskArgs:
     """The checked bpt_mask_args."""
-    if softcap is not None and not softcap > 0:
-        raise ValueError(f"softcap must be positive, got {softcap}")
+    if softcap is not None and not ctypes.c_float(softcap).value > 0:
+        raise ValueError(f"softcap must be positive as a float32, got {softcap}")
     if window is not None and window < 1:
         raise ValueError(f"window must be at least 1, got {window}")
     if slopes is not None and not (slopes.dtype == torch.float32 and tuple(slopes.shape) == (hq,) and slopes.is_contiguous()):
@@ -83,7 +83,8 @@ def paged_masked_attention(
     max_prefix   upper bound on prefix_lens, known on the host (larger ones are cut to it); sizes the launch. Default: max_context
     starts       int32 [B, Q]: each query's first token behind the prefix
     workspace, counters  optional device buffers of at least masked_plan(...) bytes, the counters zero-filled before their first
-                 use; default: cached per (device, stream), or the graph's own while one is captured
+                 use and not shared by calls that may run at once; default: cached per (device, stream), or the graph's own while
+                 one is captured
 
     Returns [B, Q, Hq, D] (or [B, Hq, D] for a 3-D q with one query per sequence) in out_dtype.
     """
@@ -116,6 +117,8 @@ def _checked(q, k_cache, v_cache, block_table, context_lens, k_scale, v_scale, s
             raise ValueError(f"out must be [{b}, {nq}, {hq}, {d}]")
         if not (out4.stride(-1) == 1 and out4.device == dev):
             raise ValueError("out must be a cuda tensor with contiguous channels")
+        if any(n > 1 and s == 0 for n, s in zip(out4.shape, out4.stride())):
+            raise ValueError("out must not be an expanded view")
     a.out = out4.data_ptr()
     a.out_stride_b, a.out_stride_q, a.out_stride_h, _ = out4.stride()
     if lse is not None:

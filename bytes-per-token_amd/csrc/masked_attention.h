@@ -410,7 +410,8 @@ __device__ __forceinline__ void masked_load_q(const MaskedParams& p, int b, int 
           const float x1 = (float)__builtin_bit_cast(_Float16, (uint16_t)(w[e] >> 16));
           const bf16x2 hi = pack_bf16(x0, x1);
           q[t][s][e] = __builtin_bit_cast(uint32_t, hi);
-          q[t][4 + s][e] = __builtin_bit_cast(uint32_t, pack_bf16(x0 - (float)hi[0], x1 - (float)hi[1]));
+          const float h0 = (float)hi[0], h1 = (float)hi[1];  // of an infinity nothing remains
+          q[t][4 + s][e] = __builtin_bit_cast(uint32_t, pack_bf16(x0 == h0 ? 0.0f : x0 - h0, x1 == h1 ? 0.0f : x1 - h1));
         }
       }
     }

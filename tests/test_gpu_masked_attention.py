@@ -244,6 +244,15 @@ def test_nan_queries_stay_in_their_row():
         assert torch.equal(got, clean)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_infinite_queries_meet_the_cap(dtype):
+    """Scores of plus and minus infinity are the cap and its negative."""
+    for nq, hq in ((2, 4), (40, 4)):
+        c = Case("bf16", False, [90], nq, hq, 2, seed=2, q_dtype=dtype)
+        c.q[0, 1, 2, 7] = float("inf")
+        c.check(softcap=2.0, out_dtype=torch.float32)
+
+
 @pytest.mark.parametrize("cap", [1e-3, 0.5, 200.0, 300.0, 1e4, 1e30])
 def test_caps_of_every_size(cap):
     """Caps past 256 take the other form of tanh; a cap far above the scores changes nothing but rounding."""
@@ -287,6 +296,12 @@ def test_views_and_outputs():
     out = buf.transpose(1, 2)[..., 3 : 3 + D]
     m.call(window=9, out=out)
     assert torch.equal(out, want) and (buf[..., :3] == 9).all() and (buf[..., 3 + D :] == 9).all()
+
+
+def test_an_expanded_output_is_refused():
+    c = Case("bf16", False, [40, 7])
+    with pytest.raises(ValueError, match="expanded"):
+        c.call(out=torch.zeros((1, *c.q.shape[1:]), device=DEV, dtype=torch.bfloat16).expand(c.q.shape))
 
 
 def test_empty_batch_and_no_context():

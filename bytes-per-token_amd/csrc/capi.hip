@@ -1029,6 +1029,7 @@ int masked_setup(const bpt_decode_args* a, const bpt_mask_args* m, const char* f
   p.max_blocks = a->max_blocks_per_seq;
   const int64_t reach = (int64_t)a->max_blocks_per_seq * a->page_size;
   p.len_cap = (int)std::min<int64_t>(a->max_context, reach);
+  if (p.len_cap > 0x7fffff00) return fail(BPT_ERR_INVALID_ARGUMENT, "%s: max_context %d too large", fn, a->max_context);  // steps end past it
   p.window = m->window >= p.len_cap ? 0 : m->window;  // a window of all tokens hides none
   p.max_prefix = m->prefix_lens ? std::min(m->max_prefix, p.len_cap) : 0;
   const double log2e = 1.4426950408889634, scale = (double)a->sm_scale * log2e;
@@ -1065,8 +1066,10 @@ int masked_setup(const bpt_decode_args* a, const bpt_mask_args* m, const char* f
   p.piece = (int)std::min<int64_t>(piece, 1 << 26);
   p.max_pieces = (int)std::max<int64_t>(1, (steps + p.piece - 1) / p.piece);
   const int64_t slots = segments * p.max_pieces;
-  if (slots > 0x70000000LL) return fail(BPT_ERR_INVALID_ARGUMENT, "%s: batch x heads x rows too large", fn);
-  plan->grid = (int)(plan->many ? slots : ((int64_t)a->batch * p.max_pieces + 7) / 8 * 8 * p.Hkv * p.tiles);  // few rows: see the kernel
+  const int64_t grid = plan->many ? slots : ((int64_t)a->batch * p.max_pieces + 7) / 8 * 8 * p.Hkv * p.tiles;  // few rows: see the kernel
+  if (grid >= 1 << 24)  // its threads are counted in 32 bits
+    return fail(BPT_ERR_INVALID_ARGUMENT, "%s: batch x heads x rows too large", fn);
+  plan->grid = (int)grid;
   plan->ws_out_floats = p.max_pieces > 1 ? (size_t)slots * p.live_rows * a->head_dim : 0;
   plan->workspace = p.max_pieces > 1 ? align256((plan->ws_out_floats + (size_t)slots * p.live_rows) * sizeof(float)) : 0;
   plan->counters = p.max_pieces > 1 ? align256((size_t)segments * sizeof(unsigned)) : 0;
@@ -1249,6 +1252,8 @@ int rotary_params(const bpt_rotary_args* a, bool pool, bpt::RotaryParams* out, b
   // longer tail. FP8 append of 4 x 4096 tokens (32 + 8 heads), 1 / 2 / 3 / 4 tokens: 117 / 98 / 103 / 99 us, INT8 of 2048: - / 60 / 66 / 68.
   const int64_t full = tokens >= 8 * bpt::kComputeUnits ? 2 : 1;
   p.tokens_per_group = (int)std::max<int64_t>(1, std::min(std::max(fill, full), most));
+  if (tokens / p.tokens_per_group >= 1 << 24)  // the launch's threads are counted in 32 bits
+    return fail(BPT_ERR_INVALID_ARGUMENT, "%s: too many tokens", fn);
   *out = p;
   return BPT_OK;
 }

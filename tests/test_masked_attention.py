@@ -27,6 +27,7 @@ def args(**change):
     (dict(prefix_lens=torch.zeros(2, dtype=torch.int32), max_prefix=-1), "max_prefix"),
     (dict(starts=torch.zeros(2, 2, dtype=torch.int32)), "starts"), (dict(starts=torch.zeros(2, 3)), "starts"),
     (dict(q=torch.zeros(2, 3, 4, 128)), "bf16 or f16"), (dict(q=torch.zeros(2, 3, 4, 64, dtype=BF)), "head_dim"), ({}, "GPU"),
+    (dict(softcap=1e-50), "softcap"),
 ])
 def test_bad_arguments_are_refused(change, said):
     from bpt_amd import paged_masked_attention
@@ -53,6 +54,7 @@ def c_args(**change):
     (dict(max_prefix=-1), "max_prefix"), (dict(head_dim=64), "head_dim"), (dict(page_size=24), "page_size"),
     (dict(sm_scale=float("nan")), "sm_scale"), (dict(softcap=1e-38, sm_scale=1e30), "out of range"),
     (dict(kv_stride_token=1 << 27), "2 GiB"), (dict(struct_size=1), "stale"),
+    (dict(max_context=2**31 - 1, max_blocks_per_seq=2**27), "max_context"),
 ])
 def test_the_c_entry_refuses(built_lib, change, said):
     from bpt_amd import _lib

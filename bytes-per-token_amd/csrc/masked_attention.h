@@ -459,16 +459,11 @@ __device__ __forceinline__ float masked_cap(float cap, float u) {
   return fmaf(-2.0f * cap, __builtin_amdgcn_rcpf(1.0f + fast_exp2(u)), cap);
 }
 
-// Scores S[rt][t] (token 16 t + 4 g + i, raw products) -> weights' two bf16 parts w[rt][part], the rows' state brought up to
-// date. sc: per-token scales of the step (keys' 32, then values' 32). careful (uniform): values that are not finite stay out of
-// the products and are added here instead (weights: this wave's 512 floats of LDS for that).
-template <int KV, int SK, int RT, bool CAREFUL>
-__device__ __forceinline__ void masked_softmax(const MaskedParams& p, const MaskedRange& rg, int b, int h, int token0, bool whole,
-                                               int lane, float qs, const float* sc, mf32x4 (&S)[RT][2], MaskedRows<RT>& st,
-                                               mu32x4 (&w)[RT][2], float* weights) {
-  const int n = lane & 15, g = lane >> 4;
-  float kf[8], vf[8];
+// Per-token scales of the lane's tokens, of a step's (keys' 32, then values' 32): keys' times qs.
+template <int SK>
+__device__ __forceinline__ void masked_scales(const float* sc, int lane, float qs, float (&kf)[8], float (&vf)[8]) {
   if constexpr (SK == kScaleTokenHead) {
+    const int g = lane >> 4;
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -477,82 +472,95 @@ __device__ __forceinline__ void masked_softmax(const MaskedParams& p, const Mask
         vf[4 * t + i] = sc[32 + 16 * t + 4 * g + i];
       }
   }
+}
+
+// Tile r's raw products S[t] (token 16 t + 4 g + i) -> scores x in log2 units, those that its row does not see (seen) at minus
+// infinity, with the row's reference point and sums brought up to date.
+template <int SK, int RT>
+__device__ __forceinline__ void masked_scores(const MaskedParams& p, const MaskedRange& rg, int token0, bool whole, int lane, float qs,
+                                              const float (&kf)[8], const mf32x4 (&S)[2], int r, MaskedRows<RT>& st, float (&x)[8],
+                                              uint32_t& seen) {
+  const int g = lane >> 4;
 #pragma unroll
-  for (int r = 0; r < RT; ++r) {
-    float x[8];
+  for (int e = 0; e < 8; ++e) x[e] = S[e >> 2][e & 3] * (SK == kScaleTokenHead ? kf[e] : qs);
+  if (p.cap > kMaskedPlainCap) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = S[r][e >> 2][e & 3] * (SK == kScaleTokenHead ? kf[e] : qs);
-    if (p.cap > kMaskedPlainCap) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {  // tanh z = z (1 - z^2 / 3 + 2 z^4 / 15 - 17 z^6 / 315) near 0, z = u ln2 / 2
-        const float z = x[e] * (0.5f * kLn2), z2 = z * z;
-        const float series = fmaf(z2, fmaf(z2, fmaf(z2, -17.0f / 315.0f, 2.0f / 15.0f), -1.0f / 3.0f), 1.0f);
-        const float y = masked_cap(p.cap, x[e]);
-        x[e] = fabsf(z) < 0.25f ? p.cap * z * series : y;
-      }
-    } else if (p.cap > 0.0f) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = masked_cap(p.cap, x[e]);
+    for (int e = 0; e < 8; ++e) {  // tanh z = z (1 - z^2 / 3 + 2 z^4 / 15 - 17 z^6 / 315) near 0, z = u ln2 / 2
+      const float z = x[e] * (0.5f * kLn2), z2 = z * z;
+      const float series = fmaf(z2, fmaf(z2, fmaf(z2, -17.0f / 315.0f, 2.0f / 15.0f), -1.0f / 3.0f), 1.0f);
+      const float y = masked_cap(p.cap, x[e]);
+      x[e] = fabsf(z) < 0.25f ? p.cap * z * series : y;
     }
-    if (p.slopes) {
-      const float d0 = (float)(st.pos[r] - token0 - 4 * g);
+  } else if (p.cap > 0.0f) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = fmaf(-st.slope[r], fabsf(d0 - (float)(16 * (e >> 2) + (e & 3))), x[e]);
-    }
-    uint32_t seen = 0xffu;
-    if (!whole) {
-      seen = 0u;
-      const int j0 = token0 + 4 * g;
+    for (int e = 0; e < 8; ++e) x[e] = masked_cap(p.cap, x[e]);
+  }
+  if (p.slopes) {
+    const float d0 = (float)(st.pos[r] - token0 - 4 * g);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int j = j0 + 16 * (e >> 2) + (e & 3);
-        const bool s = j < rg.prefix || (unsigned)(j - st.lo[r]) < (unsigned)(st.hi[r] - st.lo[r]);
-        seen |= s ? 1u << e : 0u;
-        x[e] = s ? x[e] : kNegInf;
-      }
-    }
-    float mx = x[0];
-#pragma unroll
-    for (int e = 1; e < 8; ++e) mx = fmaxf(mx, x[e]);
-    mx = max_xor<32>(max_xor<16>(mx));
-    if (__any(mx > st.m[r] + kMaskedSlack)) {  // some row's maximum left its reference point behind
-      const float m = fmaxf(st.m[r], mx);
-      const float a = st.m[r] == kNegInf ? 0.0f : fast_exp2(st.m[r] - m);
-      st.m[r] = m;
-      st.l[r] *= a;
-#pragma unroll
-      for (int c = 0; c < 8; ++c) st.o[r][c] *= a;
-    }
-    const float m = st.m[r] == kNegInf ? 0.0f : st.m[r];
-    float sum = 0.0f;
+    for (int e = 0; e < 8; ++e) x[e] = fmaf(-st.slope[r], fabsf(d0 - (float)(16 * (e >> 2) + (e & 3))), x[e]);
+  }
+  seen = 0xffu;
+  if (!whole) {
+    seen = 0u;
+    const int j0 = token0 + 4 * g;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      x[e] = fast_exp2(x[e] - m);
-      sum += x[e];
+      const int j = j0 + 16 * (e >> 2) + (e & 3);
+      const bool s = j < rg.prefix || (unsigned)(j - st.lo[r]) < (unsigned)(st.hi[r] - st.lo[r]);
+      seen |= s ? 1u << e : 0u;
+      x[e] = s ? x[e] : kNegInf;
     }
-    st.l[r] += sum;
-    if constexpr (CAREFUL) {
+  }
+  float mx = x[0];
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        weights[(16 * (e >> 2) + 4 * g + (e & 3)) * 16 + n] = (seen >> e) & 1u ? x[e] : -1.0f;
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // the wave's lanes read one another's
-      masked_add_nonfinite<KV, SK>(p, b, h, token0, rg.len, lane, weights, st.o[r]);
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    }
-    if constexpr (SK == kScaleTokenHead) {
+  for (int e = 1; e < 8; ++e) mx = fmaxf(mx, x[e]);
+  mx = max_xor<32>(max_xor<16>(mx));
+  if (__any(mx > st.m[r] + kMaskedSlack)) {  // some row's maximum left its reference point behind
+    const float m = fmaxf(st.m[r], mx);
+    const float a = st.m[r] == kNegInf ? 0.0f : fast_exp2(st.m[r] - m);
+    st.m[r] = m;
+    st.l[r] *= a;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        x[e] *= vf[e];
-        if (!whole && !((seen >> e) & 1u)) x[e] = 0.0f;  // an unseen token's scale may be anything
-        if (CAREFUL && !(fabsf(vf[e]) <= __FLT_MAX__)) x[e] = 0.0f;
-      }
-    }
+    for (int c = 0; c < 8; ++c) st.o[r][c] *= a;
+  }
+}
+
+// Tile r's scores -> weights' two bf16 parts. CAREFUL (uniform): values that are not finite stay out of the products and are added
+// here instead (weights: this wave's 512 floats of LDS for that).
+template <int KV, int SK, int RT, bool CAREFUL>
+__device__ __forceinline__ void masked_weights(const MaskedParams& p, const MaskedRange& rg, int b, int h, int token0, bool whole, int lane,
+                                               const float (&vf)[8], int r, MaskedRows<RT>& st, float (&x)[8], uint32_t seen,
+                                               mu32x4 (&w)[2], float* weights) {
+  const float m = st.m[r] == kNegInf ? 0.0f : st.m[r];
+  float sum = 0.0f;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const bf16x2 hi = pack_bf16(x[2 * e], x[2 * e + 1]);
-      w[r][0][e] = __builtin_bit_cast(uint32_t, hi);
-      w[r][1][e] = __builtin_bit_cast(uint32_t, pack_bf16(x[2 * e] - (float)hi[0], x[2 * e + 1] - (float)hi[1]));
+  for (int e = 0; e < 8; ++e) {
+    x[e] = fast_exp2(x[e] - m);
+    sum += x[e];
+  }
+  st.l[r] += sum;
+  if constexpr (CAREFUL) {
+    const int n = lane & 15, g = lane >> 4;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) weights[(16 * (e >> 2) + 4 * g + (e & 3)) * 16 + n] = (seen >> e) & 1u ? x[e] : -1.0f;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // the wave's lanes read one another's
+    masked_add_nonfinite<KV, SK>(p, b, h, token0, rg.len, lane, weights, st.o[r]);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  }
+  if constexpr (SK == kScaleTokenHead) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      x[e] *= vf[e];
+      if (!whole && !((seen >> e) & 1u)) x[e] = 0.0f;  // an unseen token's scale may be anything
+      if (CAREFUL && !(fabsf(vf[e]) <= __FLT_MAX__)) x[e] = 0.0f;
     }
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const bf16x2 hi = pack_bf16(x[2 * e], x[2 * e + 1]);
+    w[0][e] = __builtin_bit_cast(uint32_t, hi);
+    w[1][e] = __builtin_bit_cast(uint32_t, pack_bf16(x[2 * e] - (float)hi[0], x[2 * e + 1] - (float)hi[1]));
   }
 }
 
@@ -713,16 +721,21 @@ __device__ __forceinline__ void masked_few_steps(const MaskedParams& p, const Ma
         if constexpr (QS) S[0][u] = masked_mfma(f, q[0][4 + s], S[0][u]);
         S[0][u] = masked_mfma(f, q[0][s], S[0][u]);
       }
-    mu32x4 w[1][2];
-    masked_softmax<KV, SK, 1, CAREFUL>(p, rg, b, h, token0, masked_whole(rg, token0), lane, qs, w_scale, S, st, w, w_weights);
+    const bool whole = masked_whole(rg, token0);
+    float kf[8], vf[8], x[8];
+    uint32_t seen;
+    mu32x4 w[2];
+    masked_scales<SK>(w_scale, lane, qs, kf, vf);
+    masked_scores<SK, 1>(p, rg, token0, whole, lane, qs, kf, S[0], 0, st, x, seen);
+    masked_weights<KV, SK, 1, CAREFUL>(p, rg, b, h, token0, whole, lane, vf, 0, st, x, seen, w, w_weights);
 #pragma unroll
     for (int c4 = 0; c4 < 2; ++c4) {
       mu32x4 f[4];
       masked_v_frags<KV, CAREFUL>(v, c4, f);
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        st.o[0][4 * c4 + c] = masked_mfma(f[c], w[0][1], st.o[0][4 * c4 + c]);
-        st.o[0][4 * c4 + c] = masked_mfma(f[c], w[0][0], st.o[0][4 * c4 + c]);
+        st.o[0][4 * c4 + c] = masked_mfma(f[c], w[1], st.o[0][4 * c4 + c]);
+        st.o[0][4 * c4 + c] = masked_mfma(f[c], w[0], st.o[0][4 * c4 + c]);
       }
     }
     if constexpr (!last) {
@@ -896,17 +909,38 @@ __device__ __forceinline__ void masked_many_steps(const MaskedParams& p, const M
             S[r][u] = masked_mfma(f, q[r][s], S[r][u]);
           }
         }
-      mu32x4 w[RT][2];
       float* weights = s_scale + 256 + wave * kMaskedStep * 16;
-      masked_softmax<KV, SK, RT, CAREFUL>(p, mine, b, h, token0, masked_whole(mine, token0), lane, qs, s_scale + (2 * buf + u2) * 64, S, st, w,
-                                          weights);
+      const bool whole = masked_whole(mine, token0);
+      float kf[8], vf[8], x[8];
+      uint32_t seen;
+      mu32x4 w[RT][2];
+      masked_scales<SK>(s_scale + (2 * buf + u2) * 64, lane, qs, kf, vf);
+      const mu32x4* values = src + (2 + u2) * kMaskedItem + lane;
+      auto product = [&](int r, const mu32x4& v, int c) {
+        st.o[r][c] = masked_mfma(v, w[r][1], st.o[r][c]);
+        st.o[r][c] = masked_mfma(v, w[r][0], st.o[r][c]);
+      };
+      masked_scores<SK, RT>(p, mine, token0, whole, lane, qs, kf, S[0], 0, st, x, seen);
+      masked_weights<KV, SK, RT, CAREFUL>(p, mine, b, h, token0, whole, lane, vf, 0, st, x, seen, w[0], weights);
+      if constexpr (RT == 2) masked_scores<SK, RT>(p, mine, token0, whole, lane, qs, kf, S[1], 1, st, x, seen);
+      if constexpr (RT == 2 && !QS) {
+        // The first tile's products run on the matrix units while the vector units take the second's exponentials: BF16, 2048
+        // queries after 2049, capped, 122 -> 117 us, not capped 107 -> 99. An f16 q leaves no registers to hold the values.
+        mu32x4 v[8];
 #pragma unroll
-      for (int c = 0; c < 8; ++c) {
-        const mu32x4 f = src[(2 + u2) * kMaskedItem + 64 * c + lane];
+        for (int c = 0; c < 8; ++c) v[c] = values[64 * c];
 #pragma unroll
-        for (int r = 0; r < RT; ++r) {
-          st.o[r][c] = masked_mfma(f, w[r][1], st.o[r][c]);
-          st.o[r][c] = masked_mfma(f, w[r][0], st.o[r][c]);
+        for (int c = 0; c < 8; ++c) product(0, v[c], c);
+        masked_weights<KV, SK, RT, CAREFUL>(p, mine, b, h, token0, whole, lane, vf, 1, st, x, seen, w[1], weights);
+#pragma unroll
+        for (int c = 0; c < 8; ++c) product(1, v[c], c);
+      } else {
+        if constexpr (RT == 2) masked_weights<KV, SK, RT, CAREFUL>(p, mine, b, h, token0, whole, lane, vf, 1, st, x, seen, w[1], weights);
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+          const mu32x4 v = values[64 * c];
+#pragma unroll
+          for (int r = 0; r < RT; ++r) product(r, v, c);
         }
       }
     }

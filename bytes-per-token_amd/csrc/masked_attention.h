@@ -23,10 +23,12 @@
 //
 // Two kernels:
 //  * few rows (up to 48 of a KV head, in tiles of 16): the waves of a workgroup take steps in turn, straight from memory into
-//    registers, and merge through LDS at the end. Bound by the cache's bytes, short calls by the latency of a piece.
+//    registers (keys on through LDS), and merge through LDS at the end. Bound by the cache's bytes, short calls by the latency of a piece: FP8, 32
+//    sequences of 256 to 4096 tokens, 8 KV heads, 37.8 us (143 MB, 3.8 TB/s); a window of 4096 of 32768 tokens, 8 sequences, 21 us.
 //  * many rows: a workgroup's four waves hold 64 or 128 rows; each of two steps' keys and values is loaded and converted by
 //    one wave and read by all from LDS, where operands lie in the order lanes take them (no bank conflicts, no swizzle).
-//    Bound by the vector units (the scores' exponentials).
+//    Bound by the vector units, about 16 operations and 3 transcendentals (a quarter of the rate) a score: BF16, 2048 queries
+//    after 2049 tokens, 16 heads on 8, capped, window 2500, 113 us (41 GFLOP).
 //
 // Tokens a row does not see must add nothing to it, but 0 times an infinity is a NaN: a wave whose result is not finite does
 // its piece again with values that are not finite taken out of the products and added one by one to the rows that see them.
@@ -611,20 +613,26 @@ __device__ __forceinline__ void masked_store_partial(const MaskedParams& p, int6
   if (c == 0) ws_store(p.ws_lse + slot * p.live_rows + row, lse2);
 }
 
-// A tile's n pieces (slots slot0 ..) combined by the last of them to arrive, in order, so that the sum does not depend on who came
-// last: the whole workgroup of NT threads. Four pieces' loads are under way together: a round trip to the memory side takes
-// microseconds.
-template <int NT>
-__device__ __forceinline__ void masked_combine(const MaskedParams& p, int b, int h, int r0, int live, int64_t slot0, int n, int tid) {
+// A tile's n pieces (slots slot0 ..) combined by the last of them to arrive, in an order that n and the rows alone set, so that the sum
+// does not depend on who came last: the whole workgroup of NT threads. A round trip to the memory side takes a microsecond, so NP
+// pieces' loads are under way together, and where rows leave threads over, `parts` of their 16 lanes take every parts-th NP of a
+// row's pieces and meet in LDS (`lds`, 130 floats for each 16 threads): FP8, one query, 1 x 16000
+// tokens, 125 pieces of 2 rows, 45.8 -> 26.8 us (four for the few-row kernel; the many-row kernel, with registers to spare, takes eight:
+// 100 rows, 16 pieces, 53.3 -> 46.9).
+template <int NT, int NP>
+__device__ __forceinline__ void masked_combine(const MaskedParams& p, int b, int h, int r0, int live, int64_t slot0, int n, int tid,
+                                               float* lds) {
   ws_acquire();
-  constexpr int NP = 4;
-  const int c = tid & 15;
-  for (int row = tid >> 4; row < live; row += NT / 16) {
+  constexpr int GROUPS = NT / 16;
+  const int c = tid & 15, group = tid >> 4;
+  float M, W;
+  MaskedPairs o;
+  // Pieces j0 .. j0 + NP - 1 of every `step`, from `from` on: their weights' sum W and products o relative to 2^M.
+  auto fold = [&](int row, int from, int step) {
     const float* lse = p.ws_lse + slot0 * p.live_rows + row;
     const float* prt = p.ws_out + (slot0 * p.live_rows + row) * kHeadDim + 2 * c;
-    float M = kNegInf, W = 0.0f;
-    MaskedPairs o{};
-    for (int j0 = 0; j0 < n; j0 += NP) {
+    M = kNegInf, W = 0.0f, o = MaskedPairs{};
+    for (int j0 = from; j0 < n; j0 += step) {
       float lv[NP], top = kNegInf;
       MaskedPairs ov[NP];
 #pragma unroll
@@ -654,11 +662,46 @@ __device__ __forceinline__ void masked_combine(const MaskedParams& p, int b, int
       }
       M = nm;
     }
+  };
+  auto finish = [&](int row) {
     const float inv = W == 0.0f ? 0.0f : __builtin_amdgcn_rcpf(W);
 #pragma unroll
     for (int i = 0; i < 4; ++i) o.x[i][0] *= inv, o.x[i][1] *= inv;
     masked_store_pairs(p, b, h, r0 + row, c, o, W == 0.0f ? kNegInf : M + __log2f(W));
+  };
+  int parts = 1;
+  while (2 * parts * live <= GROUPS && parts * NP < n) parts *= 2;
+  if (parts == 1) {
+    for (int row = group; row < live; row += GROUPS) {
+      fold(row, 0, NP);
+      finish(row);
+    }
+    return;
   }
+  const int row = group / parts, part = group % parts;
+  float* s_mw = lds + GROUPS * kHeadDim;
+  if (row < live) {
+    fold(row, NP * part, NP * parts);
+    if (c == 0) s_mw[2 * group] = M, s_mw[2 * group + 1] = W;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) *(float2*)(lds + group * kHeadDim + 32 * i + 2 * c) = make_float2(o.x[i][0], o.x[i][1]);
+  }
+  __syncthreads();
+  if (row >= live || part != 0) return;
+  for (int s = 1; s < parts; ++s) M = fmaxf(M, s_mw[2 * (group + s)]);
+  const float mu = M == kNegInf ? 0.0f : M;
+  W = 0.0f, o = MaskedPairs{};
+  for (int s = 0; s < parts; ++s) {
+    const float m = s_mw[2 * (group + s)], w = s_mw[2 * (group + s) + 1];
+    const float a = w > 0.0f ? fast_exp2(m - mu) : (w != w ? w : 0.0f);
+    W = fmaf(a, w, W);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 x = *(const float2*)(lds + (group + s) * kHeadDim + 32 * i + 2 * c);
+      o.x[i][0] = fmaf(a, x.x, o.x[i][0]), o.x[i][1] = fmaf(a, x.y, o.x[i][1]);
+    }
+  }
+  finish(row);
 }
 
 // A workgroup's place: XCD-major (workgroups go to the 8 XCDs in turn, each with its own L2), so that the heads of a page
@@ -839,7 +882,7 @@ __global__ __launch_bounds__(256, KV == kKvBf16 ? 2 : 3) void masked_few_kernel(
   if (tid == 0) s_last = ws_arrive(p.counters + seg) == (unsigned)pieces - 1u;
   __syncthreads();
   if (!s_last) return;
-  masked_combine<256>(p, b, h, r0, live, seg * p.max_pieces, pieces, tid);
+  masked_combine<256, 4>(p, b, h, r0, live, seg * p.max_pieces, pieces, tid, smem);
   if (tid == 0) __hip_atomic_store(p.counters + seg, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
@@ -925,7 +968,7 @@ __device__ __forceinline__ void masked_many_steps(const MaskedParams& p, const M
       if constexpr (RT == 2) masked_scores<SK, RT>(p, mine, token0, whole, lane, qs, kf, S[1], 1, st, x, seen);
       if constexpr (RT == 2 && !QS) {
         // The first tile's products run on the matrix units while the vector units take the second's exponentials: BF16, 2048
-        // queries after 2049, capped, 122 -> 117 us, not capped 107 -> 99. An f16 q leaves no registers to hold the values.
+        // queries after 2049, capped, 122.7 -> 119 us, not capped 107.6 -> 99.3. An f16 q leaves no registers to hold the values.
         mu32x4 v[8];
 #pragma unroll
         for (int c = 0; c < 8; ++c) v[c] = values[64 * c];
@@ -1021,7 +1064,7 @@ __global__ __launch_bounds__(256, 2) void masked_many_kernel(const MaskedParams 
   if (tid == 0) s_last = ws_arrive(p.counters + seg) == (unsigned)pieces - 1u;
   __syncthreads();
   if (!s_last) return;
-  masked_combine<256>(p, b, h, r0, live, seg * p.max_pieces, pieces, tid);
+  masked_combine<256, 8>(p, b, h, r0, live, seg * p.max_pieces, pieces, tid, s_o);
   if (tid == 0) __hip_atomic_store(p.counters + seg, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
@@ -1034,6 +1077,7 @@ static hipError_t launch_masked_t(const MaskedParams& p, int rt, bool many, int 
   const size_t merge = (size_t)4 * live * (kMaskedRowPad + 2) * sizeof(float);
   const size_t early = (size_t)(16 * masked_key_units(KV) + 4 * 64 + 4 * kMaskedStep * 16) * sizeof(float);
   const size_t few = merge > early ? merge : early;
+  static_assert((16 * masked_key_units(KV) + 4 * 64) >= 16 * (kHeadDim + 2), "the combine's shares fit");
   hipError_t e = hipSuccess;
   auto run = [&](auto kernel, size_t lds) {
     if (lds > (64u << 10))  // has to be asked for, once per device

@@ -150,6 +150,29 @@ def test_split_over_many_pieces(fmt, per_token, nq, hq):
     c.check(window=700, prefix_lens=i32([130, 1, 2000]))
 
 
+@pytest.mark.parametrize("nq, hq", [(1, 2), (1, 4), (1, 6), (1, 10), (1, 16), (1, 18), (2, 20), (100, 2)])
+@pytest.mark.parametrize("mask", ["causal", "steep", "prefix"])
+def test_long_sequences_of_few_heads(nq, hq, mask):
+    """Dozens of pieces a row, shared out among the threads that combine them where there are few rows."""
+    c = Case("fp8", False, [9000, 2100], nq, hq, 2, seed=hq)
+    how = {"causal": {}, "steep": dict(slopes=torch.full((hq,), 0.3, device=DEV)),
+           "prefix": dict(prefix_lens=i32([100, 2100]), starts=torch.full((2, nq), 8500, device=DEV, dtype=torch.int32))}[mask]
+    c.check(out_dtype=torch.float32, **how)
+    once = c.call(**how)
+    assert torch.equal(once, c.call(**how))
+
+
+def test_nan_reaches_its_row_through_many_pieces():
+    for hq in (2, 10):
+        c = Case("bf16", False, [9000], 1, hq, 2, seed=2)
+        clean = c.call()
+        c.q[0, 0, 1, 7] = float("nan")
+        got = c.call()
+        assert torch.isnan(got[0, 0, 1]).all()
+        got[0, 0, 1] = clean[0, 0, 1]
+        assert torch.equal(got, clean)
+
+
 def test_pieces_are_combined_in_order():
     """The same call gives the same bits, whichever piece comes last."""
     c = Case("fp8", False, [9000, 8000, 77], 2, 8, 2)

@@ -23,8 +23,9 @@
 //
 // Two kernels:
 //  * few rows (up to 48 of a KV head, in tiles of 16): the waves of a workgroup take steps in turn, straight from memory into
-//    registers (keys on through LDS), and merge through LDS at the end. Bound by the cache's bytes, short calls by the latency of a piece: FP8, 32
-//    sequences of 256 to 4096 tokens, 8 KV heads, 37.8 us (143 MB, 3.8 TB/s); a window of 4096 of 32768 tokens, 8 sequences, 21 us.
+//    registers (keys on through LDS), and merge through LDS at the end. Bound by the cache's bytes, short calls by the latency
+//    of a piece: FP8, 32 sequences of 256 to 4096 tokens, 8 KV heads, 37.8 us (143 MB, 3.8 TB/s); a window of 4096 of 32768
+//    tokens, 8 sequences, 21 us.
 //  * many rows: a workgroup's four waves hold 64 or 128 rows; each of two steps' keys and values is loaded and converted by
 //    one wave and read by all from LDS, where operands lie in the order lanes take them (no bank conflicts, no swizzle).
 //    Bound by the vector units, about 16 operations and 3 transcendentals (a quarter of the rate) a score: BF16, 2048 queries
@@ -301,7 +302,8 @@ struct MaskedRange {
 __device__ __forceinline__ int masked_token0(const MaskedRange& r, int t) { return kMaskedStep * (t < r.sa ? t : r.sb + t - r.sa); }
 
 // The page ids of step t's two 16-token groups, in lanes 0 and 1, and of step t + stride's, in lanes 2 and 3 (both clamped to the
-// piece's last step), on their way for masked_pages. (Scalar loads would share their counter with LDS: every read of that would wait for the page table.)
+// piece's last step), on their way for masked_pages. (Scalar loads would share their counter with LDS: every read of that would
+// wait for the page table.)
 template <bool PU>
 __device__ __forceinline__ int masked_page_list(const MaskedParams& p, const MaskedRange& r, int b, int t, int stride, int t1, int lane) {
   if (!PU) return 0;
@@ -613,12 +615,12 @@ __device__ __forceinline__ void masked_store_partial(const MaskedParams& p, int6
   if (c == 0) ws_store(p.ws_lse + slot * p.live_rows + row, lse2);
 }
 
-// A tile's n pieces (slots slot0 ..) combined by the last of them to arrive, in an order that n and the rows alone set, so that the sum
-// does not depend on who came last: the whole workgroup of NT threads. A round trip to the memory side takes a microsecond, so NP
-// pieces' loads are under way together, and where rows leave threads over, `parts` of their 16 lanes take every parts-th NP of a
-// row's pieces and meet in LDS (`lds`, 130 floats for each 16 threads): FP8, one query, 1 x 16000
-// tokens, 125 pieces of 2 rows, 45.8 -> 26.8 us (four for the few-row kernel; the many-row kernel, with registers to spare, takes eight:
-// 100 rows, 16 pieces, 53.3 -> 46.9).
+// A tile's n pieces (slots slot0 ..) combined by the last of them to arrive, in an order that n and the rows alone set, so that
+// the sum does not depend on who came last: the whole workgroup of NT threads. A round trip to the memory side takes a
+// microsecond, so NP pieces' loads are under way together (four for the few-row kernel; eight for the many-row one, which has the
+// registers: 100 rows, 16 pieces, 53.3 -> 46.9 us), and where rows leave threads over, `parts` of their 16 lanes take every
+// parts-th NP of a row's pieces and meet in LDS (`lds`, 130 floats for each 16 threads): FP8, one query, 1 x 16000 tokens, 125
+// pieces of 2 rows, 45.8 -> 26.8 us.
 template <int NT, int NP>
 __device__ __forceinline__ void masked_combine(const MaskedParams& p, int b, int h, int r0, int live, int64_t slot0, int n, int tid,
                                                float* lds) {
@@ -716,9 +718,9 @@ constexpr int masked_key_units(int kv) { return kMaskedStep * (kv == kKvBf16 ? 1
 
 // ---- few rows ---------------------------------------------------------------------------------------------------
 
-// One wave's steps t, t + 4, ... < t1 folded into its rows (list: the page ids of the first two). The next step's keys are requested once this one's have gone to LDS,
-// its values once this one's are multiplied, and the page ids of the step after that in between: no request stands behind a
-// branch, so that each is waited for by itself.
+// One wave's steps t, t + 4, ... < t1 folded into its rows (list: the page ids of the first two). The next step's keys are requested
+// once this one's have gone to LDS, its values once this one's are multiplied, and the page ids of the step after that in between:
+// no request stands behind a branch, so that each is waited for by itself.
 template <int KV, int SK, bool PU, bool QS, bool ONCE, bool CAREFUL>
 __device__ __forceinline__ void masked_few_steps(const MaskedParams& p, const MaskedRange& rg, int b, int h, int t, int t1, int lane,
                                                  float qs, const mu32x4 (&q)[1][QS ? 8 : 4], int list, mu32x4* w_keys,

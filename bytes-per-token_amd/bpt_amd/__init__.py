@@ -3,10 +3,10 @@
 The decode hot path of fastserve (kernels/kv_attention.py, engine/kv_cache.py, integration/kv_cache.py),
 re-implemented as hand-written HIP kernels behind a C ABI (include/bpt_amd.h, built into libbpt_amd.so)
 with a thin PyTorch-ROCm host layer: paged FP8 / INT8 / BF16 pools (paged_attention, kv_cache) and
-contiguous KIVI caches (kivi: fastserve's kernels/kv_attention.py call surface), and the fused RMSNorm +
-per-token INT8 quantizer (norm_quant: kernels/norm_quant.py), and rotary positions on the way into the paged cache
-(rotary) and attention with masked and shaped scores over it (masked_attention). Importing needs no GPU; the library loads on first use and raises if
-it has not been built.
+contiguous KIVI caches (kivi: fastserve's kernels/kv_attention.py call surface), the fused RMSNorm +
+per-token INT8 quantizer (norm_quant: kernels/norm_quant.py), rotary positions on the way into the paged cache
+(rotary), and attention with masked and shaped scores over it (masked_attention). Importing needs no GPU; the
+library loads on first use and raises if it has not been built.
 """
 
 from . import kivi
